@@ -103,6 +103,9 @@ SIGNATURES = {
     "bt_dynamic_quantize_ranged": (ctypes.c_int, [_P(BtTensor), _P(BtTensor), ctypes.c_void_p, ctypes.c_void_p,
                                                   ctypes.c_void_p]),
     "bt_conv_int_epilogue": (ctypes.c_int, [_P(BtTensor)] * 5),
+    "bt_quantize_rows": (ctypes.c_int, [_P(BtTensor)] * 3),
+    "bt_matmul_int8": (ctypes.c_int, [_P(BtTensor)] * 6),
+    "bt_attention": (ctypes.c_int, [_P(BtTensor)] * 5 + [ctypes.c_float, _P(BtTensor)]),
 }
 
 _lib = None

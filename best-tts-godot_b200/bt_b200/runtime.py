@@ -30,6 +30,8 @@ library raises ``BtError`` (a RuntimeError).
 """
 import ctypes
 import functools
+import math
+import threading
 import weakref
 
 import numpy as np
@@ -166,6 +168,7 @@ class BtRuntime:
         self._ew_plans = {}
         self._node_plans = {}   # node signature -> launch plan (see dispatch)
         self._scalars = {}
+        self._local = threading.local()   # per-thread launch plans (see _thread_plans)
         self.launches = 0
 
     # ---- device values ---------------------------------------------------------
@@ -763,6 +766,208 @@ class BtRuntime:
         self.launches += 1
         return out
 
+    # ---- quantised projections and attention -----------------------------------------
+    def _thread_plans(self):
+        """This thread's launch plans.  A plan's descriptors receive the data
+        pointers of each call, so threads do not share them."""
+        try:
+            return self._local.plans
+        except AttributeError:
+            self._local.plans = plans = {}
+            return plans
+
+    def _keep_plan(self, plans, key, plan):
+        if len(plans) >= 4096:
+            plans.clear()
+        plans[key] = plan
+        return plan
+
+    def _check_here(self, what, **tensors):
+        for name, t in tensors.items():
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{what}: {name} must be a CUDA tensor, not {type(t).__name__}")
+            if t.get_device() != self._index:
+                raise ValueError(f"{what}: {name} is on {t.device}, this runtime on {self.device}")
+
+    def _call(self, fn, what, *args):
+        """A library call on this runtime's device and the current stream."""
+        if torch.cuda.current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self._call(fn, what, *args)
+        self.lib.bt_set_stream(_raw_stream(self._index))   # always BT_OK
+        rc = fn(*args)
+        if rc:
+            check(rc, what)
+        self.launches += 1
+
+    def quantize_rows(self, x):
+        """Symmetric 8-bit rows (bt_quantize_rows): for x [..., K] float32 /
+        float16, (q int8 of x's shape, scale float32 of shape x.shape[:-1])
+        with q * scale[..., None] ~ x: each row's largest magnitude becomes
+        127.  Rows of activations are tokens, rows of a weight [N, K] are
+        output channels.  q's rows start on 16-byte boundaries (a view of a
+        wider buffer where K is not a multiple of 16), as matmul_int8 reads
+        them in place."""
+        self._check_here("quantize_rows", x=x)
+        plans = self._thread_plans()
+        key = ("quantize_rows", x.dtype, x.shape, x.stride())
+        plan = plans.get(key)
+        if plan is None:
+            if x.dtype not in (torch.float32, torch.float16):
+                raise TypeError(f"quantize_rows: x must be float32 or float16, not {x.dtype}")
+            if x.dim() < 1 or x.shape[-1] == 0:
+                raise ValueError("quantize_rows: rows without values have no largest value")
+            if not _one_row_stride(x):
+                return self.quantize_rows(self._contig(x))
+            K = int(x.shape[-1])
+            lead = tuple(int(s) for s in x.shape[:-1])
+            padded = (K + 15) // 16 * 16
+            rows = math.prod(lead)
+            xd = tensor_desc(x)
+            qd = make_tensor(0, np.int8, (rows, K), (padded, 1))
+            plan = self._keep_plan(plans, key, (xd, qd, make_tensor(0, np.float32, (rows,)), lead, padded, K, rows))
+        xd, qd, sd, lead, padded, K, rows = plan
+        q = torch.empty(lead + (padded,), dtype=torch.int8, device=self.device)
+        scale = torch.empty(lead, dtype=torch.float32, device=self.device)
+        if rows:
+            xd.data, qd.data, sd.data = x.data_ptr(), q.data_ptr(), scale.data_ptr()
+            self._call(self.lib.bt_quantize_rows, "bt_quantize_rows", xd, qd, sd)
+        return (q if padded == K else q[..., :K]), scale
+
+    def matmul_int8(self, a, a_scale, w, w_scale, bias=None, out_dtype=torch.float32):
+        """The product of 8-bit rows with a scale for each token and output
+        channel (bt_matmul_int8): a int8 [..., K] with a_scale float32 of
+        shape a.shape[:-1], w int8 [N, K] with w_scale float32 [N] (both as
+        quantize_rows returns them), bias float32 [N] or None; returns
+        (sum_k a w) * a_scale * w_scale + bias as float32 or float16
+        [..., N].  The integer sum is exact.  Operands whose rows do not
+        start on 16-byte boundaries are copied to such rows first."""
+        self._check_here("matmul_int8", a=a, a_scale=a_scale, w=w, w_scale=w_scale)
+        if bias is not None:
+            self._check_here("matmul_int8", bias=bias)
+        plans = self._thread_plans()
+        key = ("matmul_int8", a.dtype, a.shape, a.stride(), a_scale.dtype, a_scale.shape, a_scale.stride(), w.dtype,
+               w.shape, w.stride(), w_scale.dtype, w_scale.shape, w_scale.stride(),
+               None if bias is None else (bias.dtype, bias.shape, bias.stride()), out_dtype)
+        plan = plans.get(key)
+        if plan is None:
+            plan = self._keep_plan(plans, key, self._matmul_int8_plan(a, a_scale, w, w_scale, bias, out_dtype))
+        ad, asd, wd, wsd, bd, od, shape, fits = plan
+        if not fits or (a.data_ptr() | w.data_ptr()) & 15:
+            a2, w2 = self._aligned_rows(a), self._aligned_rows(w)
+            s2 = a_scale if a_scale.is_contiguous() else self._contig(a_scale)
+            if a2 is not a or w2 is not w or s2 is not a_scale:
+                return self.matmul_int8(a2, s2, w2, w_scale, bias, out_dtype)
+        out = torch.empty(shape, dtype=out_dtype, device=self.device)
+        if out.numel():
+            ad.data, asd.data, wd.data, wsd.data = a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr()
+            od.data = out.data_ptr()
+            if bias is not None:
+                bd.data = bias.data_ptr()
+            self._call(self.lib.bt_matmul_int8, "bt_matmul_int8", ad, asd, wd, wsd, bd, od)
+        return out
+
+    def _matmul_int8_plan(self, a, a_scale, w, w_scale, bias, out_dtype):
+        what = "matmul_int8"
+        if a.dtype != torch.int8 or w.dtype != torch.int8:
+            raise TypeError(f"{what}: a and w must be int8, not {a.dtype} and {w.dtype}")
+        for name, t in (("a_scale", a_scale), ("w_scale", w_scale), ("bias", bias)):
+            if t is not None and t.dtype != torch.float32:
+                raise TypeError(f"{what}: {name} must be float32, not {t.dtype}")
+        if out_dtype not in (torch.float32, torch.float16):
+            raise TypeError(f"{what}: out_dtype must be float32 or float16, not {out_dtype}")
+        if a.dim() < 1 or w.dim() != 2 or a.shape[-1] != w.shape[1]:
+            raise ValueError(f"{what}: a [..., K] and w [N, K] of shapes {tuple(a.shape)} and {tuple(w.shape)}")
+        N, K = (int(v) for v in w.shape)
+        lead = tuple(int(s) for s in a.shape[:-1])
+        if K > 131071:
+            raise ValueError(f"{what}: more than 131071 values a row could overflow the int32 sum")
+        if tuple(a_scale.shape) != lead:
+            raise ValueError(f"{what}: a_scale of shape {tuple(a_scale.shape)} for rows {lead}")
+        for name, t in (("w_scale", w_scale), ("bias", bias)):
+            if t is not None and tuple(t.shape) != (N,):
+                raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} for {N} output channels")
+        rows = math.prod(lead)
+        fits = _row_pitch_ok(a) and _row_pitch_ok(w) and a_scale.is_contiguous()
+        dt = TORCH_TO_NP[out_dtype]
+        return (tensor_desc(a), make_tensor(0, np.float32, (rows,)), tensor_desc(w), tensor_desc(w_scale),
+                None if bias is None else tensor_desc(bias), make_tensor(0, dt, (rows, N)), lead + (N,), fits)
+
+    def _aligned_rows(self, t):
+        """t itself where its rows have one stride, a multiple of 16 bytes,
+        and start on 16-byte boundaries; else a copy laid out so."""
+        if _row_pitch_ok(t) and t.data_ptr() & 15 == 0:
+            return t
+        lead, K = tuple(t.shape[:-1]), int(t.shape[-1])
+        buf = torch.empty(lead + ((K + 15) // 16 * 16,), dtype=t.dtype, device=self.device)
+        return self._copy_desc(tensor_desc(t), np_dtype(t), buf[..., :K])
+
+    def attention(self, q, k, v, lengths=None, key_mask=None, scale=None):
+        """softmax(scale * q k^T) v (bt_attention) of queries q [B, H, Tq, D]
+        over keys and values k, v [B, Hk, Tk, D] of another length, float32
+        or float16 (scores and sums in float32 either way); returns q's shape
+        and dtype in q's axis order.  Query head h reads key head
+        h // (H / Hk).  lengths: int32 / int64 [B], the keys of each batch
+        entry (default: all); key_mask: bool [B, Tk], true where a key takes
+        part; keys that do not are never looked at, and a row without any
+        gives zeros.  scale defaults to 1 / sqrt(D).  Views of any strides
+        are read in place (a [B, T, H, D] projection permuted to
+        [B, H, T, D])."""
+        self._check_here("attention", q=q, k=k, v=v)
+        if lengths is not None:
+            self._check_here("attention", lengths=lengths)
+        if key_mask is not None:
+            self._check_here("attention", key_mask=key_mask)
+        plans = self._thread_plans()
+        key = ("attention", q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(),
+               None if lengths is None else (lengths.dtype, lengths.shape, lengths.stride()),
+               None if key_mask is None else (key_mask.dtype, key_mask.shape, key_mask.stride()),
+               scale)
+        plan = plans.get(key)
+        if plan is None:
+            plan = self._keep_plan(plans, key, self._attention_plan(q, k, v, lengths, key_mask, scale))
+        qd, kd, vd, ld, md, od, sc, shape, strides = plan
+        out = torch.empty_strided(shape, strides, dtype=q.dtype, device=self.device)
+        if out.numel():
+            qd.data, kd.data, vd.data, od.data = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+            if lengths is not None:
+                ld.data = lengths.data_ptr()
+            if key_mask is not None:
+                md.data = key_mask.data_ptr()
+            self._call(self.lib.bt_attention, "bt_attention", qd, kd, vd, ld, md, sc, od)
+        return out
+
+    def _attention_plan(self, q, k, v, lengths, key_mask, scale):
+        what = "attention"
+        if q.dtype not in (torch.float32, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError(f"{what}: q, k and v must all be float32 or all float16, not {q.dtype}, {k.dtype}, {v.dtype}")
+        if q.dim() != 4 or k.dim() != 4 or tuple(k.shape) != tuple(v.shape):
+            raise ValueError(f"{what}: q [B, H, Tq, D], k and v [B, Hk, Tk, D] of shapes {tuple(q.shape)}, "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        B, H, _, D = (int(s) for s in q.shape)
+        Hk, Tk = int(k.shape[1]), int(k.shape[2])
+        if k.shape[0] != B or k.shape[3] != D or (H % Hk if Hk else H):
+            raise ValueError(f"{what}: q of shape {tuple(q.shape)} cannot attend to k of shape {tuple(k.shape)}")
+        scale = 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale)
+        if lengths is not None:
+            if lengths.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"{what}: lengths must be int32 or int64, not {lengths.dtype}")
+            if tuple(lengths.shape) != (B,):
+                raise ValueError(f"{what}: lengths of shape {tuple(lengths.shape)} for batch {B}")
+        if key_mask is not None:
+            if key_mask.dtype != torch.bool:
+                raise TypeError(f"{what}: key_mask must be bool, not {key_mask.dtype}")
+            if tuple(key_mask.shape) != (B, Tk):
+                raise ValueError(f"{what}: key_mask of shape {tuple(key_mask.shape)} for keys [{B}, {Tk}]")
+        shape = tuple(int(s) for s in q.shape)
+        order, strides, acc = _k_order([q], shape), [0] * 4, 1
+        for ax in reversed(order):
+            strides[ax] = acc
+            acc *= shape[ax]
+        od = make_tensor(0, np_dtype(q), shape, strides)
+        return (tensor_desc(q), tensor_desc(k), tensor_desc(v), None if lengths is None else tensor_desc(lengths),
+                None if key_mask is None else tensor_desc(key_mask), od, scale, shape, tuple(strides))
+
     def _as_f32(self, t):
         dt = np_dtype(t)
         if dt == np.float32:
@@ -1174,6 +1379,30 @@ def _axis_blocks(axes, shape):
                 continue
         blocks.append([a])
     return blocks
+
+
+def _one_row_stride(t):
+    """Whether t's leading axes collapse to one axis of constant stride over
+    rows of unit stride (rows of a C-contiguous tensor, or of a wider buffer)."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return False
+    n = 1
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] != 1:
+            if n == 1:
+                step = t.stride(d)
+            elif t.stride(d) != step * n:
+                return False
+            n *= int(t.shape[d])
+    return True
+
+
+def _row_pitch_ok(t):
+    """Rows of one stride that is a multiple of 16 bytes."""
+    if not _one_row_stride(t):
+        return False
+    step = next((t.stride(d) for d in range(t.dim() - 2, -1, -1) if t.shape[d] != 1), 0)
+    return step * t.element_size() % 16 == 0
 
 
 def _host_ints(v):

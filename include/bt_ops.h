@@ -330,6 +330,50 @@ int bt_conv_int_epilogue(const bt_tensor* acc, const bt_tensor* bias,
                          const bt_tensor* x_scale, const bt_tensor* w_scale,
                          const bt_tensor* out);
 
+/* ---- quantised projections -------------------------------------------------
+ * Symmetric 8-bit rows: for each row of x (float32 or float16; all leading
+ * axes, the last axis of unit stride), in float32 with one rounding a step,
+ *   a = max(max |x|, 2^-100),  scale = a / 127,  q = rint(x * (127 / a)).
+ * rint rounds half to even.  A row with a NaN gets a NaN scale and one with
+ * an infinity an infinite scale; a NaN product becomes 0.  q int8 of x's
+ * shape (rows of one stride, unit stride inside), scale float32 [rows].
+ * Rows without values are BT_ESHAPE.
+ * No counterpart in the reference, whose DynamicQuantizeLinear
+ * (ref_runtime.py:106-116) has one scale for the whole tensor. */
+int bt_quantize_rows(const bt_tensor* x, const bt_tensor* q,
+                     const bt_tensor* scale);
+/* The product of int8 rows with a scale for each token and output channel:
+ *   out[m, n] = sum_k a[m, k] w[n, k] * (a_scale[m] * w_scale[n]) [+ bias[n]]
+ * a int8 [..., K] (M rows), w int8 [N, K] (one row per output channel),
+ * a_scale [M], w_scale [N] and bias [N] (NULL: none) float32, out float32 or
+ * float16 [..., N].  The sum is an exact int32; it is converted to float32,
+ * scaled, biased, and rounded to float16 once where out is float16.  K at
+ * most 131071 (beyond it the sum could overflow: BT_ETOOBIG); K = 0 gives
+ * the bias, or 0.
+ * No counterpart in the reference, whose MatMulInteger nodes have one
+ * activation scale for the whole tensor. */
+int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
+                   const bt_tensor* w, const bt_tensor* w_scale,
+                   const bt_tensor* bias, const bt_tensor* out);
+
+/* ---- attention ---------------------------------------------------------------
+ * out = softmax(scale * q k^T) v for queries q [B, H, Tq, D] over keys and
+ * values k, v [B, Hk, Tk, D] of another length (an encoder's states, or the
+ * queries' own sequence); query head h reads key head h / (H / Hk), so H is a
+ * multiple of Hk.  One dtype for q, k, v and out: float32 or float16; any
+ * strides (a permuted [B, T, H, D] projection is read in place); D at most
+ * 128.  lengths (NULL: Tk): int32 or int64 [B], the keys of each batch entry,
+ * clamped to 0..Tk.  key_mask (NULL: none): bool [B, Tk], true where a key
+ * takes part.  Keys that do not take part are never looked at, whatever their
+ * k and v rows hold; a query row no key takes part in gives zeros.  scale:
+ * positive and finite.  Scores, softmax and sums are float32.
+ * replaces: the MatMul, Mul, Add, Softmax, MatMul nodes of an attention block
+ *           (ref_runtime.py:446-451, :269-273 + :599-600 for Mul, Add and
+ *           Softmax), one dispatch each in the reference. */
+int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_tensor* v,
+                 const bt_tensor* lengths, const bt_tensor* key_mask,
+                 float scale, const bt_tensor* out);
+
 /* ---- host-only helpers (no GPU) ------------------------------------------ */
 /* Broadcast-and-collapse planner used by bt_elementwise: merges adjacent axes
  * that every operand walks contiguously and drops size-1 axes (the behaviour
