@@ -1398,11 +1398,12 @@ def _one_row_stride(t):
 
 
 def _row_pitch_ok(t):
-    """Rows of one stride that is a multiple of 16 bytes."""
+    """Rows of one stride, a multiple of 16 bytes above 0 (a broadcast row
+    has none)."""
     if not _one_row_stride(t):
         return False
-    step = next((t.stride(d) for d in range(t.dim() - 2, -1, -1) if t.shape[d] != 1), 0)
-    return step * t.element_size() % 16 == 0
+    step = next((t.stride(d) for d in range(t.dim() - 2, -1, -1) if t.shape[d] != 1), 16)
+    return step > 0 and step * t.element_size() % 16 == 0
 
 
 def _host_ints(v):

@@ -806,9 +806,9 @@ int adain_v3(const bt_adain_args* p, uint32_t* const* range) {
 
 extern "C" int bt_wait_timeouts(uint32_t* count) {
   if (!count) return bt::set_error(BT_EINVAL, "bt_wait_timeouts: null count");
-  unsigned int v = 0, zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbol(&v, bt::g_bulk_timeouts, sizeof(v));
-  if (e == cudaSuccess) e = cudaMemcpyToSymbol(bt::g_bulk_timeouts, &zero, sizeof(zero));
+  unsigned int v = 0;
+  cudaError_t e = bt::take_timeouts(&v);
+  if (e == cudaSuccess) e = bt::proj_timeouts(&v);
   if (e != cudaSuccess) return bt::set_error(BT_ECUDA, "bt_wait_timeouts: %s", cudaGetErrorString(e));
   *count = v;
   return BT_OK;

@@ -12,13 +12,24 @@
 // g_bulk_timeouts and returns, so a copy that never completes shows as an
 // error instead of a hung kernel.  The counter has internal linkage (the
 // library is built without relocatable device code): each translation unit
-// that waits on bulk copies exports a reader of its own (bt_wait_timeouts).
+// that waits on copies has its own, which take_timeouts reads and resets;
+// bt_wait_timeouts adds them up.
 #pragma once
 #include <stdint.h>
+#include <cuda_runtime.h>
 
 namespace bt {
 namespace {
 __device__ unsigned int g_bulk_timeouts = 0;
+
+// Adds this translation unit's count on the current device and resets it.
+[[maybe_unused]] cudaError_t take_timeouts(unsigned int* sum) {
+  unsigned int v = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_bulk_timeouts, sizeof(v));
+  if (e == cudaSuccess && v) e = cudaMemcpyToSymbol(g_bulk_timeouts, &zero, sizeof(zero));
+  *sum += v;
+  return e;
+}
 }  // namespace
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }

@@ -3,9 +3,11 @@
 // and each output channel (bt_matmul_int8).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 #include "bt_ops.h"
 #include "bt_internal.h"
+#include "bt_tc.h"
 
 namespace bt {
 namespace {
@@ -71,29 +73,363 @@ struct MmArgs {
   int64_t sa, sw, sb;  // strides of the scales and the bias
 };
 
+// K = 0: the sum is empty.
 template <typename TO>
-__global__ void __launch_bounds__(256) matmul_int8_kernel(MmArgs A) {
-  __shared__ int8_t as[16][33], ws[16][33];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t n_tiles = (A.N + 15) / 16;
-  const int64_t m0 = (int64_t)blockIdx.x / n_tiles * 16, n0 = (int64_t)blockIdx.x % n_tiles * 16;
-  int acc = 0;
-  for (int64_t k0 = 0; k0 < A.K; k0 += 32) {
-    for (int i = threadIdx.x; i < 512; i += 256) {
-      const int r = i >> 5, c = i & 31;
-      as[r][c] = m0 + r < A.M && k0 + c < A.K ? A.a[(m0 + r) * A.lda + k0 + c] : (int8_t)0;
-      ws[r][c] = n0 + r < A.N && k0 + c < A.K ? A.w[(n0 + r) * A.ldw + k0 + c] : (int8_t)0;
-    }
-    __syncthreads();
-    for (int c = 0; c < 32; ++c) acc += (int)as[ty][c] * (int)ws[tx][c];
-    __syncthreads();
+__global__ void __launch_bounds__(256) matmul_empty_kernel(MmArgs A) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < A.M * A.N; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / A.N, n = i % A.N;
+    float y = __fmul_rn(0.0f, __fmul_rn(A.a_scale[m * A.sa], A.w_scale[n * A.sw]));
+    if (A.bias) y = __fadd_rn(y, A.bias[n * A.sb]);
+    if constexpr (sizeof(TO) == 2) ((__half*)A.out)[m * A.ldo + n] = __float2half_rn(y);
+    else ((float*)A.out)[m * A.ldo + n] = y;
   }
-  const int64_t m = m0 + ty, n = n0 + tx;
-  if (m >= A.M || n >= A.N) return;
-  float y = __fmul_rn(__int2float_rn(acc), __fmul_rn(A.a_scale[m * A.sa], A.w_scale[n * A.sw]));
-  if (A.bias) y = __fadd_rn(y, A.bias[n * A.sb]);
-  if constexpr (sizeof(TO) == 2) ((__half*)A.out)[m * A.ldo + n] = __float2half_rn(y);
-  else ((float*)A.out)[m * A.ldo + n] = y;
+}
+
+// The product on the tensor cores.  Output channels lie along the 128 lanes
+// of tensor memory and tokens along its columns: one token is enough to use
+// the instruction (a tile of 16 columns), a thread owns one channel, so its
+// scale and bias sit in registers, and the 32 lanes of a warp store 32
+// neighbouring channels of one token.
+//
+// A unit -- one CTA (CG = 1), or a pair whose instruction spans both SMs
+// (CG = 2) -- walks tiles of 128 * CG channels x NT tokens.  Warp 0 loads
+// 128-byte-wide blocks of both operands by TMA into a ring of stages (the
+// pair splits the tokens, so each SM loads and reads half of them), warp 1
+// issues the matrix instructions, warps 2-5 scale and store from one of two
+// accumulators while the next tile fills the other.
+//
+// Where a product has fewer tiles than the GPU has SMs, S CTAs form a cluster
+// that splits the summed axis of one tile; each sends its int32 partial sums
+// to the CTA that owns the column (shared memory of the cluster), which adds
+// and stores them.  Integer sums do not depend on the order.
+template <int NT, int CG>
+struct MmShape {
+  static constexpr int kA = 128 * 128;              // bytes of one stage: channels
+  static constexpr int kB = NT / CG * 128;          // and tokens
+  static constexpr int kStage = kA + kB;
+  static constexpr int kStages = 200 * 1024 / kStage > 8 ? 8 : 200 * 1024 / kStage;
+  static constexpr int kBufs = 2;
+  static constexpr int kCols = NT * kBufs < 32 ? 32 : NT * kBufs;   // tensor memory
+  static constexpr int kSmem = kStages * kStage + 1024 + 512 + NT * 4 * kBufs;
+};
+
+template <typename TO>
+__device__ __forceinline__ void mm_store(TO* p, float v) {
+  if constexpr (sizeof(TO) == 2) *p = __float2half_rn(v);
+  else *p = v;
+}
+
+__device__ __forceinline__ void mm_tile(const MmArgs& A, int64_t t, int64_t tiles_n, int64_t tiles_m, int64_t* tn,
+                                        int64_t* tm) {
+  // bands of eight channel tiles, so that the tiles in flight share both
+  // operands' rows in L2
+  const int64_t band = t / (8 * tiles_m), r = t - band * 8 * tiles_m;
+  const int64_t width = tiles_n - band * 8 < 8 ? tiles_n - band * 8 : 8;
+  *tm = r / width;
+  *tn = band * 8 + r % width;
+}
+
+template <int NT, int CG, typename TO>
+__global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                           const __grid_constant__ CUtensorMap map_a, MmArgs A,
+                                                           int S) {
+  using Sh = MmShape<NT, CG>;
+  extern __shared__ uint8_t smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* ring = smem_raw + (base - smem_u32(smem_raw));
+  uint64_t* full = (uint64_t*)(ring + Sh::kStages * Sh::kStage);
+  uint64_t* empty = full + Sh::kStages;
+  uint64_t* acc_full = empty + Sh::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* slot = (uint32_t*)(acc_empty + 2);
+  volatile int* aborted = (volatile int*)(slot + 1);
+  float* tok_scale = (float*)(full + 64);   // [2][NT]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned csize = CG == 2 ? 2 : (unsigned)S;
+  const unsigned rank = csize > 1 ? cluster_rank() : 0;
+  const bool leader = CG == 1 || rank == 0;
+  const int64_t unit = blockIdx.x / csize, units = gridDim.x / csize;
+  const int64_t tiles_n = (A.N + 128 * CG - 1) / (128 * CG), tiles_m = (A.M + NT - 1) / NT;
+  const int64_t tiles = tiles_n * tiles_m;
+  const int kblocks = (int)((A.K + 127) / 128);
+  const int kb0 = CG == 1 ? (int)((int64_t)kblocks * rank / S) : 0;
+  const int kb1 = CG == 1 ? (int)((int64_t)kblocks * (rank + 1) / S) : kblocks;
+
+  if (threadIdx.x == 0) {
+    *aborted = 0;
+    for (int i = 0; i < Sh::kStages; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 4 * CG);
+    }
+    tma_prefetch(&map_w);
+    tma_prefetch(&map_a);
+  }
+  if (warp == 1) tmem_alloc<CG>(slot, Sh::kCols);
+  tc_fence_before();
+  __syncthreads();
+  if (csize > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int st = 0;
+      unsigned ph = 0;
+      for (int64_t t = unit; t < tiles; t += units) {
+        int64_t tn, tm;
+        mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
+        const int n0 = (int)(tn * 128 * CG + (CG == 2 ? 128 * rank : 0));
+        const int m0 = (int)(tm * NT + (CG == 2 ? NT / 2 * rank : 0));
+        for (int kb = kb0; kb < kb1; ++kb) {
+          tc_wait(empty + st, ph ^ 1, aborted);
+          const unsigned dst = base + st * Sh::kStage;
+          if (leader) mbar_arrive_expect_tx(full + st, Sh::kStage * CG);
+          if constexpr (CG == 1) {
+            tma_load2(dst, &map_w, smem_u32(full + st), kb * 128, n0);
+            tma_load2(dst + Sh::kA, &map_a, smem_u32(full + st), kb * 128, m0);
+          } else {
+            const unsigned bar = cluster_addr(smem_u32(full + st), 0);
+            tma_load2_pair(dst, &map_w, bar, kb * 128, n0);
+            tma_load2_pair(dst + Sh::kA, &map_a, bar, kb * 128, m0);
+          }
+          if (++st == Sh::kStages) st = 0, ph ^= 1;
+        }
+      }
+      // every stage drained: no arrival is under way when the CTA ends
+      for (int i = 0; i < Sh::kStages; ++i) {
+        tc_wait(empty + st, ph ^ 1, aborted);
+        if (++st == Sh::kStages) st = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // int32 accumulator, signed 8-bit operands, both K-major
+      constexpr uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (NT / 8u) << 17 | (128u * CG / 16u) << 24;
+      int st = 0, buf = 0;
+      unsigned ph = 0, aph = 0;
+      for (int64_t t = unit; t < tiles; t += units) {
+        tc_wait(acc_empty + buf, aph ^ 1, aborted);
+        tc_fence_after();
+        const uint32_t d = tmem + buf * NT;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          tc_wait(full + st, ph, aborted);
+          tc_fence_after();
+          const unsigned sa = base + st * Sh::kStage, sb = sa + Sh::kA;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_i8<CG>(d, smem_desc(sa + 32 * k, 16, 1024), smem_desc(sb + 32 * k, 16, 1024), idesc, kb > kb0 || k > 0);
+          if constexpr (CG == 1) mma_commit(empty + st);
+          else mma_commit_pair(empty + st);
+          if (++st == Sh::kStages) st = 0, ph ^= 1;
+        }
+        if constexpr (CG == 1) mma_commit(acc_full + buf);
+        else mma_commit_pair(acc_full + buf);
+        if (++buf == 2) buf = 0, aph ^= 1;
+      }
+    }
+  } else {
+    const int quad = warp & 3, et = threadIdx.x - 64;
+    int buf = 0;
+    unsigned aph = 0;
+    for (int64_t t = unit; t < tiles; t += units) {
+      int64_t tn, tm;
+      mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
+      if (CG == 1 && S > 1) {
+        tc_wait(acc_full + buf, aph, aborted);   // (the cluster finishes below)
+        continue;
+      }
+      const int64_t n = tn * 128 * CG + (CG == 2 ? 128 * rank : 0) + quad * 32 + lane, m0 = tm * NT;
+      const int cols = A.M - m0 < NT ? (int)(A.M - m0) : NT;
+      float* ts = tok_scale + buf * NT;
+      // (the previous use of this half was two tiles ago: every warp has
+      // passed the barrier of the tile between)
+      for (int i = et; i < cols; i += 128) ts[i] = A.a_scale[(m0 + i) * A.sa];
+      const bool live = n < A.N;
+      const float sw = live ? A.w_scale[n * A.sw] : 0.0f, b = live && A.bias ? A.bias[n * A.sb] : 0.0f;
+      const bool biased = A.bias != nullptr;
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+      tc_wait(acc_full + buf, aph, aborted);
+      tc_fence_after();
+      TO* op = (TO*)A.out + m0 * A.ldo + n;
+      constexpr int CH = NT < 32 ? 16 : 32;
+#pragma unroll 1
+      for (int c0 = 0; c0 < NT; c0 += CH) {
+        if (c0 >= cols) break;
+        uint32_t r[CH];
+        if constexpr (CH == 32) tmem_ld32(tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16), r);
+        else tmem_ld16(tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16), r);
+        tc_wait_ld();
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            if (c0 + j < cols) {
+              float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(ts[c0 + j], sw));
+              if (biased) y = __fadd_rn(y, b);
+              mm_store(op + (int64_t)(c0 + j) * A.ldo, y);
+            }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 1) mbar_arrive(acc_empty + buf);
+        else mbar_arrive_cluster(cluster_addr(smem_u32(acc_empty + buf), 0));
+      }
+      if (++buf == 2) buf = 0, aph ^= 1;
+    }
+  }
+  __syncwarp();
+  if constexpr (CG == 1) {
+    if (S > 1) {
+      // every CTA of the cluster has its partial sums; the rings are free
+      tc_fence_before();
+      __syncthreads();
+      cluster_arrive();
+      cluster_wait();
+      tc_fence_after();
+      const int per = (NT + S - 1) / S;
+      int64_t tn, tm;
+      mm_tile(A, unit, tiles_n, tiles_m, &tn, &tm);
+      const int64_t m0 = tm * NT;
+      const int cols = A.M - m0 < NT ? (int)(A.M - m0) : NT;
+      if (warp >= 2) {
+        const int quad = warp & 3;
+        constexpr int CH = NT < 32 ? 16 : 32;
+#pragma unroll 1
+        for (int c0 = 0; c0 < cols; c0 += CH) {
+          uint32_t r[CH];
+          if constexpr (CH == 32) tmem_ld32(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
+          else tmem_ld16(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const int c = c0 + j, owner = c % S;
+            if (c < cols) {
+              const unsigned a = cluster_addr(base + ((rank * per + c / S) * 128 + quad * 32 + lane) * 4, owner);
+              asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(a), "r"(r[j]) : "memory");
+            }
+          }
+        }
+      }
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      if (warp >= 2) {
+        const int ch = threadIdx.x - 64;
+        const int64_t n = tn * 128 + ch;
+        if (n < A.N) {
+          const float sw = A.w_scale[n * A.sw], b = A.bias ? A.bias[n * A.sb] : 0.0f;
+          const int* red = (const int*)ring;
+          for (int c = rank, i = 0; c < cols; c += S, ++i) {
+            int acc = 0;
+            for (int s = 0; s < S; ++s) acc += red[(s * per + i) * 128 + ch];
+            float y = __fmul_rn(__int2float_rn(acc), __fmul_rn(A.a_scale[(m0 + c) * A.sa], sw));
+            if (A.bias) y = __fadd_rn(y, b);
+            mm_store((TO*)A.out + (m0 + c) * A.ldo + n, y);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*aborted) {   // copies may still be in flight: give them time to land
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) {}
+  }
+  __syncwarp();
+  if constexpr (CG == 2) {   // the pair's last instructions and arrivals are done on both sides
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (warp == 1) tmem_free<CG>(tmem, Sh::kCols);
+}
+
+template <int NT, int CG, typename TO>
+int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
+  using Sh = MmShape<NT, CG>;
+  CUtensorMap mw, ma;
+  const uint64_t dw[2] = {(uint64_t)A.K, (uint64_t)A.N}, da[2] = {(uint64_t)A.K, (uint64_t)A.M};
+  const uint64_t sw[1] = {(uint64_t)A.ldw}, sa[1] = {(uint64_t)A.lda};
+  const uint32_t bw[2] = {128, 128}, ba[2] = {128, (uint32_t)(NT / CG)};
+  int rc;
+  if ((rc = tma_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.w, dw, sw, bw)) ||
+      (rc = tma_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.a, da, sa, ba)))
+    return rc;
+  auto kern = matmul_tc_kernel<NT, CG, TO>;
+  static int raised[64] = {};   // per device: the limit only has to be raised once
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !raised[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    if (e != cudaSuccess) return set_error(BT_ECUDA, "%s: shared memory: %s", what, cudaGetErrorString(e));
+    if (dev < 64) raised[dev] = 1;
+  }
+  const int64_t tiles = (A.N + 128 * CG - 1) / (128 * CG) * ((A.M + NT - 1) / NT);
+  const int csize = CG == 2 ? 2 : S;
+  const int64_t cap = S > 1 ? tiles : sms / CG;
+  const int64_t units = tiles < cap ? tiles : cap;
+  if (units * csize > INT32_MAX) return set_error(BT_ETOOBIG, "%s: too many output values", what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * csize));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = Sh::kSmem;
+  cfg.stream = cur_stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)csize, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, A, S);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(BT_ECUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+  }
+  return BT_OK;
+}
+
+template <typename TO>
+int mm_run(const MmArgs& A, int sms, const char* what) {
+  // The tile and the split with the least estimated time, in SM clocks: a
+  // block of 128 along the summed axis takes the longer of its matrix
+  // instructions (8192 products a clock) and its loads (64 bytes a clock);
+  // a tile adds its stores, a launch its start, a split its exchange.
+  const int kblocks = (int)((A.K + 127) / 128);
+  int best_nt = 0, best_cg = 1, best_s = 1;
+  double best = 1e300;
+  auto consider = [&](int nt, int cg, int s) {
+    const double tiles = (double)((A.N + 128 * cg - 1) / (128 * cg)) * (double)((A.M + nt - 1) / nt);
+    const double units = cg == 2 ? sms / 2 : sms / s;
+    const double waves = ceil(tiles / units);
+    const double mma = 2.0 * nt, load = (16384 + nt * 128 / cg) / 64.0;
+    const double per = ceil((double)kblocks / s) * (mma > load ? mma : load);
+    const double store = nt * 8.0;
+    const double t = 3000 + waves * (per > store ? per : store) + store + (s > 1 ? 2500 + 20.0 * nt : 0);
+    if (t < best) best = t, best_nt = nt, best_cg = cg, best_s = s;
+  };
+  for (int nt = 16; nt <= 256; nt *= 2) {
+    if (nt > 16 && A.M <= nt / 2) break;
+    consider(nt, 1, 1);
+    if (nt <= 128)
+      for (int s = 2; s <= 8 && s <= kblocks; ++s) consider(nt, 1, s);
+  }
+  consider(256, 2, 1);
+  if (best_cg == 2) return mm_launch<256, 2, TO>(A, 1, sms, what);
+  switch (best_nt) {
+    case 16: return mm_launch<16, 1, TO>(A, best_s, sms, what);
+    case 32: return mm_launch<32, 1, TO>(A, best_s, sms, what);
+    case 64: return mm_launch<64, 1, TO>(A, best_s, sms, what);
+    case 128: return mm_launch<128, 1, TO>(A, best_s, sms, what);
+    default: return mm_launch<256, 1, TO>(A, best_s, sms, what);
+  }
 }
 
 // The rows of a view: all leading axes as one axis of constant stride, the
@@ -130,6 +466,9 @@ int vec_of(const bt_tensor* t, const char* what, const char* name, int64_t n, co
 }
 
 }  // namespace
+
+cudaError_t proj_timeouts(unsigned int* sum) { return take_timeouts(sum); }
+
 }  // namespace bt
 
 using namespace bt;
@@ -190,9 +529,21 @@ extern "C" int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale, cons
   A.a = (const int8_t*)a->data;
   A.w = (const int8_t*)w->data;
   A.out = out->data;
-  const int64_t tiles = (A.M + 15) / 16 * ((A.N + 15) / 16);
-  if (tiles > INT32_MAX) return set_error(BT_ETOOBIG, "%s: too many output values", what);
-  if (out->dtype == BT_F32) matmul_int8_kernel<float><<<(int)tiles, 256, 0, cur_stream()>>>(A);
-  else matmul_int8_kernel<__half><<<(int)tiles, 256, 0, cur_stream()>>>(A);
-  return check_launch(what);
+  DevInfo di;
+  if (A.K == 0) {
+    if ((rc = dev_info(&di))) return rc;
+    const int64_t want = (A.M * A.N + 255) / 256, cap = (int64_t)di.sm_count * 8;
+    const int grid = (int)(want < cap ? want : cap);
+    if (out->dtype == BT_F32) matmul_empty_kernel<float><<<grid, 256, 0, cur_stream()>>>(A);
+    else matmul_empty_kernel<__half><<<grid, 256, 0, cur_stream()>>>(A);
+    return check_launch(what);
+  }
+  if (A.M > INT32_MAX - 256 || A.N > INT32_MAX - 256) return set_error(BT_ETOOBIG, "%s: more than 2^31 rows", what);
+  // one row has no stride to speak of: any that a tensor map takes
+  if (A.M == 1) A.lda = (A.K + 15) / 16 * 16;
+  if (A.N == 1) A.ldw = (A.K + 15) / 16 * 16;
+  if ((((uintptr_t)A.a | (uintptr_t)A.w) & 15) || A.lda <= 0 || A.ldw <= 0 || (A.lda & 15) || (A.ldw & 15))
+    return set_error(BT_EUNSUPPORTED, "%s: the rows of a and w must start on 16-byte boundaries", what);
+  if ((rc = dev_info(&di))) return rc;
+  return out->dtype == BT_F32 ? mm_run<float>(A, di.sm_count, what) : mm_run<__half>(A, di.sm_count, what);
 }

@@ -238,3 +238,12 @@ def test_streams_threads_and_graphs(gpu_runtime):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, rt.matmul_int8(*rt.quantize_rows(x), w, sw, bias=b))
+
+
+def test_no_wait_gave_up(gpu_runtime):
+    """Every bounded wait of the runs above ended by what it waited for."""
+    import ctypes
+    from bt_b200._lib import check
+    n = ctypes.c_uint32(99)
+    check(gpu_runtime.lib.bt_wait_timeouts(ctypes.byref(n)), "bt_wait_timeouts")
+    assert n.value == 0
