@@ -95,8 +95,10 @@ __global__ void __launch_bounds__(256) matmul_empty_kernel(MmArgs A) {
 // (CG = 2) -- walks tiles of 128 * CG channels x NT tokens.  Warp 0 loads
 // 128-byte-wide blocks of both operands by TMA into a ring of stages (the
 // pair splits the tokens, so each SM loads and reads half of them), warp 1
-// issues the matrix instructions, warps 2-5 scale and store from one of two
-// accumulators while the next tile fills the other.
+// issues the matrix instructions, warps 2-9 scale and store from one of two
+// accumulators while the next tile fills the other: a warp turns 32 channels
+// x kChunk tokens into rows of shared memory and hands them to a TMA store,
+// or, where out's rows are not on 16-byte boundaries, stores them directly.
 //
 // Where a product has fewer tiles than the GPU has SMs, S CTAs form a cluster
 // that splits the summed axis of one tile; each sends its int32 partial sums
@@ -107,11 +109,12 @@ struct MmShape {
   static constexpr int kA = 128 * 128;              // bytes of one stage: channels
   static constexpr int kB = NT / CG * 128;          // and tokens
   static constexpr int kStage = kA + kB;
-  static constexpr int kStages = 200 * 1024 / kStage > 8 ? 8 : 200 * 1024 / kStage;
-  static constexpr int kBufs = 2;
-  static constexpr int kCols = NT * kBufs < 32 ? 32 : NT * kBufs;   // tensor memory
-  static constexpr int kSmem = kStages * kStage + 1024 + 512 + NT * 4 * kBufs;
+  static constexpr int kStages = 192 * 1024 / kStage > 8 ? 8 : 192 * 1024 / kStage;
+  static constexpr int kCols = 2 * NT;              // tensor memory: two accumulators
+  static constexpr int kOut = 8 * 2 * 2048;         // two store buffers for each of eight warps
+  static constexpr int kSmem = 1024 + kStages * kStage + kOut + 512;
 };
+constexpr int kMmThreads = 320;
 
 template <typename TO>
 __device__ __forceinline__ void mm_store(TO* p, float v) {
@@ -130,20 +133,20 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, int64_t t, int64_t tile
 }
 
 template <int NT, int CG, typename TO>
-__global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant__ CUtensorMap map_w,
-                                                           const __grid_constant__ CUtensorMap map_a, MmArgs A,
-                                                           int S) {
+__global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_constant__ CUtensorMap map_w,
+                                                           const __grid_constant__ CUtensorMap map_a,
+                                                           const __grid_constant__ CUtensorMap map_out, MmArgs A,
+                                                           int S, int tma_out) {
   using Sh = MmShape<NT, CG>;
   extern __shared__ uint8_t smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* ring = smem_raw + (base - smem_u32(smem_raw));
-  uint64_t* full = (uint64_t*)(ring + Sh::kStages * Sh::kStage);
+  uint64_t* full = (uint64_t*)(ring + Sh::kStages * Sh::kStage + Sh::kOut);
   uint64_t* empty = full + Sh::kStages;
   uint64_t* acc_full = empty + Sh::kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* slot = (uint32_t*)(acc_empty + 2);
   volatile int* aborted = (volatile int*)(slot + 1);
-  float* tok_scale = (float*)(full + 64);   // [2][NT]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned csize = CG == 2 ? 2 : (unsigned)S;
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 4 * CG);
+      mbar_init(acc_empty + i, 8 * CG);
     }
     tma_prefetch(&map_w);
     tma_prefetch(&map_a);
@@ -236,45 +239,78 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
       }
     }
   } else {
-    const int quad = warp & 3, et = threadIdx.x - 64;
-    int buf = 0;
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    // two warps share a quarter of the lanes, each takes every other chunk
+    constexpr int kChunk = sizeof(TO) == 2 ? 32 : 16;
+    constexpr int kFirst = NT / kChunk >= 2 ? 2 : 1;   // chunks a warp steps over
+    const unsigned stage_out = base + Sh::kStages * Sh::kStage + (warp - 2) * 4096;
+    int buf = 0, ob = 0;
     unsigned aph = 0;
     for (int64_t t = unit; t < tiles; t += units) {
-      int64_t tn, tm;
-      mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
       if (CG == 1 && S > 1) {
         tc_wait(acc_full + buf, aph, aborted);   // (the cluster finishes below)
         continue;
       }
-      const int64_t n = tn * 128 * CG + (CG == 2 ? 128 * rank : 0) + quad * 32 + lane, m0 = tm * NT;
-      const int cols = A.M - m0 < NT ? (int)(A.M - m0) : NT;
-      float* ts = tok_scale + buf * NT;
-      // (the previous use of this half was two tiles ago: every warp has
-      // passed the barrier of the tile between)
-      for (int i = et; i < cols; i += 128) ts[i] = A.a_scale[(m0 + i) * A.sa];
+      int64_t tn, tm;
+      mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
+      const int64_t n0 = tn * 128 * CG + (CG == 2 ? 128 * rank : 0) + quad * 32, n = n0 + lane, m0 = tm * NT;
+      const int cols = n0 >= A.N ? 0 : A.M - m0 < NT ? (int)(A.M - m0) : NT;
       const bool live = n < A.N;
       const float sw = live ? A.w_scale[n * A.sw] : 0.0f, b = live && A.bias ? A.bias[n * A.sb] : 0.0f;
       const bool biased = A.bias != nullptr;
-      asm volatile("bar.sync 1, 128;\n" ::: "memory");
+      int c0 = half * kChunk;
+      // lane i holds token c0 + i's scale
+      float ts = lane < kChunk && c0 + lane < cols ? A.a_scale[(m0 + c0 + lane) * A.sa] : 0.0f;
       tc_wait(acc_full + buf, aph, aborted);
       tc_fence_after();
-      TO* op = (TO*)A.out + m0 * A.ldo + n;
-      constexpr int CH = NT < 32 ? 16 : 32;
 #pragma unroll 1
-      for (int c0 = 0; c0 < NT; c0 += CH) {
-        if (c0 >= cols) break;
-        uint32_t r[CH];
-        if constexpr (CH == 32) tmem_ld32(tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16), r);
-        else tmem_ld16(tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16), r);
-        tc_wait_ld();
-        if (live) {
+      for (; c0 < cols; c0 += kFirst * kChunk) {
+        uint32_t r[kChunk];
+        const uint32_t at = tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16);
+        if constexpr (kChunk == 32 && NT < 32) {
+          uint32_t q[16];
+          tmem_ld16(at, q);
 #pragma unroll
-          for (int j = 0; j < CH; ++j)
-            if (c0 + j < cols) {
-              float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(ts[c0 + j], sw));
-              if (biased) y = __fadd_rn(y, b);
-              mm_store(op + (int64_t)(c0 + j) * A.ldo, y);
-            }
+          for (int j = 0; j < 32; ++j) r[j] = j < 16 ? q[j & 15] : 0;
+        } else if constexpr (kChunk == 32) {
+          tmem_ld32(at, r);
+        } else {
+          tmem_ld16(at, r);
+        }
+        const float now = ts;
+        const int next = c0 + kFirst * kChunk + lane;
+        ts = lane < kChunk && next < cols ? A.a_scale[(m0 + next) * A.sa] : 0.0f;
+        tc_wait_ld();
+        if (tma_out) {
+          const unsigned rows = stage_out + ob * 2048;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(__shfl_sync(0xffffffffu, now, j), sw));
+            if (biased) y = __fadd_rn(y, b);
+            if constexpr (sizeof(TO) == 2)
+              asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(rows + j * 64 + lane * 2), "h"(__half_as_ushort(__float2half_rn(y)))
+                           : "memory");
+            else
+              asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(rows + j * 128 + lane * 4), "f"(y) : "memory");
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store2(&map_out, rows, (int)n0, (int)(m0 + c0));
+            bulk_commit();
+          }
+          ob ^= 1;
+        } else {
+          TO* op = (TO*)A.out + (m0 + c0) * A.ldo + n;
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(__shfl_sync(0xffffffffu, now, j), sw));
+            if (biased) y = __fadd_rn(y, b);
+            if (live && c0 + j < cols) mm_store(op, y);
+            op += A.ldo;
+          }
         }
       }
       tc_fence_before();
@@ -285,6 +321,7 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
       }
       if (++buf == 2) buf = 0, aph ^= 1;
     }
+    if (lane == 0) bulk_wait_all();
   }
   __syncwarp();
   if constexpr (CG == 1) {
@@ -302,12 +339,11 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
       const int cols = A.M - m0 < NT ? (int)(A.M - m0) : NT;
       if (warp >= 2) {
         const int quad = warp & 3;
-        constexpr int CH = NT < 32 ? 16 : 32;
+        constexpr int CH = 16;
 #pragma unroll 1
-        for (int c0 = 0; c0 < cols; c0 += CH) {
+        for (int c0 = ((warp - 2) >> 2) * CH; c0 < cols; c0 += 2 * CH) {
           uint32_t r[CH];
-          if constexpr (CH == 32) tmem_ld32(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
-          else tmem_ld16(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
+          tmem_ld16(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
@@ -323,12 +359,12 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
       cluster_arrive();
       cluster_wait();
       if (warp >= 2) {
-        const int ch = threadIdx.x - 64;
+        const int ch = (threadIdx.x - 64) & 127, first = (warp - 2) >> 2;
         const int64_t n = tn * 128 + ch;
         if (n < A.N) {
           const float sw = A.w_scale[n * A.sw], b = A.bias ? A.bias[n * A.sb] : 0.0f;
           const int* red = (const int*)ring;
-          for (int c = rank, i = 0; c < cols; c += S, ++i) {
+          for (int i = first, c = rank + first * S; c < cols; c += 2 * S, i += 2) {
             int acc = 0;
             for (int s = 0; s < S; ++s) acc += red[(s * per + i) * 128 + ch];
             float y = __fmul_rn(__int2float_rn(acc), __fmul_rn(A.a_scale[(m0 + c) * A.sa], sw));
@@ -356,7 +392,7 @@ __global__ void __launch_bounds__(192, 1) matmul_tc_kernel(const __grid_constant
 template <int NT, int CG, typename TO>
 int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   using Sh = MmShape<NT, CG>;
-  CUtensorMap mw, ma;
+  CUtensorMap mw, ma, mo = {};
   const uint64_t dw[2] = {(uint64_t)A.K, (uint64_t)A.N}, da[2] = {(uint64_t)A.K, (uint64_t)A.M};
   const uint64_t sw[1] = {(uint64_t)A.ldw}, sa[1] = {(uint64_t)A.lda};
   const uint32_t bw[2] = {128, 128}, ba[2] = {128, (uint32_t)(NT / CG)};
@@ -364,6 +400,15 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   if ((rc = tma_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.w, dw, sw, bw)) ||
       (rc = tma_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.a, da, sa, ba)))
     return rc;
+  const int64_t pitch = A.ldo * (int64_t)sizeof(TO);
+  const int tma_out = S == 1 && ((uintptr_t)A.out & 15) == 0 && (A.M == 1 || (pitch > 0 && pitch % 16 == 0));
+  if (tma_out) {
+    const uint64_t d[2] = {(uint64_t)A.N, (uint64_t)A.M}, st[1] = {(uint64_t)(A.M == 1 ? (A.N + 7) / 8 * 32 : pitch)};
+    const uint32_t box[2] = {32, (uint32_t)(sizeof(TO) == 2 ? (NT < 32 ? NT : 32) : 16)};
+    if ((rc = tma_map(&mo, sizeof(TO) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, A.out, d,
+                      st, box, false)))
+      return rc;
+  }
   auto kern = matmul_tc_kernel<NT, CG, TO>;
   static int raised[64] = {};   // per device: the limit only has to be raised once
   int dev = 0;
@@ -380,7 +425,7 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   if (units * csize > INT32_MAX) return set_error(BT_ETOOBIG, "%s: too many output values", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * csize));
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(kMmThreads);
   cfg.dynamicSmemBytes = Sh::kSmem;
   cfg.stream = cur_stream();
   cudaLaunchAttribute at[1];
@@ -388,7 +433,7 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   at[0].val.clusterDim = {(unsigned)csize, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, A, S);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, mo, A, S, tma_out);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(BT_ECUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));

@@ -19,10 +19,11 @@
 namespace bt {
 
 // ---- host: tensor maps -------------------------------------------------------
-// A tiled map over `rank` axes, innermost first, of 128-byte swizzled boxes;
-// strides in bytes for axes 1.. .  Returns a status.
+// A tiled map over `rank` axes, innermost first, of 128-byte swizzled boxes
+// (loads) or plain ones (stores); strides in bytes for axes 1.. .  Returns a
+// status.
 int tma_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
-            const uint64_t* strides, const uint32_t* box);
+            const uint64_t* strides, const uint32_t* box, bool swizzle = true);
 
 // ---- device ------------------------------------------------------------------
 constexpr long long kWaitCycles = 4000000000ll;   // about two seconds
@@ -89,6 +90,19 @@ __device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap* m, un
       "[%2];\n" ::"r"(dst),
       "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
+}
+
+// Shared memory -> the box at (x, y), clipped to the map's extents, in this
+// thread's current bulk group.
+__device__ __forceinline__ void tma_store2(const CUtensorMap* m, unsigned src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(m), "r"(src), "r"(x),
+               "r"(y)
+               : "memory");
+}
+// Until at most N of this thread's bulk groups still read shared memory.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
