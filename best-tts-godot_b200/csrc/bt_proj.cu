@@ -95,26 +95,32 @@ __global__ void __launch_bounds__(256) matmul_empty_kernel(MmArgs A) {
 // (CG = 2) -- walks tiles of 128 * CG channels x NT tokens.  Warp 0 loads
 // 128-byte-wide blocks of both operands by TMA into a ring of stages (the
 // pair splits the tokens, so each SM loads and reads half of them), warp 1
-// issues the matrix instructions, warps 2-9 scale and store from one of two
-// accumulators while the next tile fills the other: a warp turns 32 channels
-// x kChunk tokens into rows of shared memory and hands them to a TMA store,
-// or, where out's rows are not on 16-byte boundaries, stores them directly.
+// issues the matrix instructions, sixteen further warps scale and store from
+// one of two accumulators while the next tile fills the other.  That pass is
+// bound by its chain of steps, not by the stores: with eight warps the
+// batched projection (32640 x 2048 x 768, float16) took 69 us, and turning
+// the tile round in shared memory for whole-row or TMA stores changed
+// nothing (67-71 us).
 //
 // Where a product has fewer tiles than the GPU has SMs, S CTAs form a cluster
 // that splits the summed axis of one tile; each sends its int32 partial sums
 // to the CTA that owns the column (shared memory of the cluster), which adds
 // and stores them.  Integer sums do not depend on the order.
+constexpr int kMmStore = 16, kMmThreads = 64 + 32 * kMmStore;   // storing warps: four for each quarter of the lanes
+
 template <int NT, int CG>
 struct MmShape {
   static constexpr int kA = 128 * 128;              // bytes of one stage: channels
   static constexpr int kB = NT / CG * 128;          // and tokens
   static constexpr int kStage = kA + kB;
-  static constexpr int kStages = 192 * 1024 / kStage > 8 ? 8 : 192 * 1024 / kStage;
+  static constexpr int kStages = 200 * 1024 / kStage > 8 ? 8 : 200 * 1024 / kStage;
   static constexpr int kCols = 2 * NT;              // tensor memory: two accumulators
-  static constexpr int kOut = 8 * 2 * 2048;         // two store buffers for each of eight warps
-  static constexpr int kSmem = 1024 + kStages * kStage + kOut + 512;
+  static constexpr int kChunk = NT < 64 ? 16 : 32;  // columns a storing warp takes at a time
+  static constexpr int kTok = NT <= 128 ? 32 : NT / 4;   // scales it keeps for its tokens
+  static constexpr int kScales = kMmStore * kTok * 4;
+  static constexpr int kSmem = 1024 + kStages * kStage + kScales + 512;
 };
-constexpr int kMmThreads = 320;
+
 
 template <typename TO>
 __device__ __forceinline__ void mm_store(TO* p, float v) {
@@ -122,26 +128,56 @@ __device__ __forceinline__ void mm_store(TO* p, float v) {
   else *p = v;
 }
 
-__device__ __forceinline__ void mm_tile(const MmArgs& A, int64_t t, int64_t tiles_n, int64_t tiles_m, int64_t* tn,
-                                        int64_t* tm) {
+// kChunk columns of an accumulator.
+template <int kChunk>
+__device__ __forceinline__ void mm_ld(uint32_t at, uint32_t (&r)[kChunk]) {
+  if constexpr (kChunk == 16) tmem_ld16(at, r);
+  else tmem_ld32(at, r);
+}
+
+__device__ __forceinline__ void mm_tile(unsigned t, unsigned tiles_n, unsigned tiles_m, int* tn, int* tm) {
   // bands of eight channel tiles, so that the tiles in flight share both
   // operands' rows in L2
-  const int64_t band = t / (8 * tiles_m), r = t - band * 8 * tiles_m;
-  const int64_t width = tiles_n - band * 8 < 8 ? tiles_n - band * 8 : 8;
-  *tm = r / width;
-  *tn = band * 8 + r % width;
+  const unsigned band = t / (8 * tiles_m), r = t - band * 8 * tiles_m;
+  const unsigned width = tiles_n - band * 8 < 8 ? tiles_n - band * 8 : 8, m = r / width;
+  *tm = (int)m;
+  *tn = (int)(band * 8 + r - m * width);
 }
+
+// Where a storing warp's part of a tile lies and the scales it needs: its
+// channel's, and its tokens' spread over the lanes.  Chunk i of warp group g
+// is tokens [(4 i + g) kChunk, + kChunk) of the tile.
+template <int NT, int CG>
+struct MmTile {
+  static constexpr int kTok = MmShape<NT, CG>::kTok / 32, kChunk = MmShape<NT, CG>::kChunk;
+  int64_t m0, n0;
+  float sw, b, tok[kTok];
+  __device__ __forceinline__ void load(const MmArgs& A, unsigned t, unsigned tiles_n, unsigned tiles_m, unsigned rank,
+                                       int quad, int group, int lane) {
+    int tn, tm;
+    mm_tile(t, tiles_n, tiles_m, &tn, &tm);
+    m0 = (int64_t)tm * NT;
+    n0 = (int64_t)tn * 128 * CG + (CG == 2 ? 128 * (int)rank : 0) + quad * 32;
+    const int64_t n = n0 + lane;
+    sw = n < A.N ? A.w_scale[n * A.sw] : 0.0f;
+    b = n < A.N && A.bias ? A.bias[n * A.sb] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kTok; ++k) {
+      const int i = lane + 32 * k, c = (i / kChunk * 4 + group) * kChunk + i % kChunk;
+      tok[k] = c < NT && m0 + c < A.M ? A.a_scale[(m0 + c) * A.sa] : 0.0f;
+    }
+  }
+};
 
 template <int NT, int CG, typename TO>
 __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_constant__ CUtensorMap map_w,
                                                            const __grid_constant__ CUtensorMap map_a,
-                                                           const __grid_constant__ CUtensorMap map_out, MmArgs A,
-                                                           int S, int tma_out) {
+                                                           MmArgs A, int S) {
   using Sh = MmShape<NT, CG>;
   extern __shared__ uint8_t smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* ring = smem_raw + (base - smem_u32(smem_raw));
-  uint64_t* full = (uint64_t*)(ring + Sh::kStages * Sh::kStage + Sh::kOut);
+  uint64_t* full = (uint64_t*)(ring + Sh::kStages * Sh::kStage + Sh::kScales);
   uint64_t* empty = full + Sh::kStages;
   uint64_t* acc_full = empty + Sh::kStages;
   uint64_t* acc_empty = acc_full + 2;
@@ -152,9 +188,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
   const unsigned csize = CG == 2 ? 2 : (unsigned)S;
   const unsigned rank = csize > 1 ? cluster_rank() : 0;
   const bool leader = CG == 1 || rank == 0;
-  const int64_t unit = blockIdx.x / csize, units = gridDim.x / csize;
-  const int64_t tiles_n = (A.N + 128 * CG - 1) / (128 * CG), tiles_m = (A.M + NT - 1) / NT;
-  const int64_t tiles = tiles_n * tiles_m;
+  const unsigned unit = blockIdx.x / csize, units = gridDim.x / csize;
+  const unsigned tiles_n = (unsigned)((A.N + 128 * CG - 1) / (128 * CG)), tiles_m = (unsigned)((A.M + NT - 1) / NT);
+  const unsigned tiles = tiles_n * tiles_m;   // (the host keeps tiles + units below 2^31)
   const int kblocks = (int)((A.K + 127) / 128);
   const int kb0 = CG == 1 ? (int)((int64_t)kblocks * rank / S) : 0;
   const int kb1 = CG == 1 ? (int)((int64_t)kblocks * (rank + 1) / S) : kblocks;
@@ -167,7 +203,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + i, 1);
-      mbar_init(acc_empty + i, 8 * CG);
+      mbar_init(acc_empty + i, kMmStore * CG);
     }
     tma_prefetch(&map_w);
     tma_prefetch(&map_a);
@@ -186,11 +222,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
     if (lane == 0) {
       int st = 0;
       unsigned ph = 0;
-      for (int64_t t = unit; t < tiles; t += units) {
-        int64_t tn, tm;
-        mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
-        const int n0 = (int)(tn * 128 * CG + (CG == 2 ? 128 * rank : 0));
-        const int m0 = (int)(tm * NT + (CG == 2 ? NT / 2 * rank : 0));
+      for (unsigned t = unit; t < tiles; t += units) {
+        int tn, tm;
+        mm_tile(t, tiles_n, tiles_m, &tn, &tm);
+        const int n0 = tn * 128 * CG + (CG == 2 ? 128 * (int)rank : 0);
+        const int m0 = tm * NT + (CG == 2 ? NT / 2 * (int)rank : 0);
         for (int kb = kb0; kb < kb1; ++kb) {
           tc_wait(empty + st, ph ^ 1, aborted);
           const unsigned dst = base + st * Sh::kStage;
@@ -218,7 +254,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       constexpr uint32_t idesc = 2u << 4 | 1u << 7 | 1u << 10 | (NT / 8u) << 17 | (128u * CG / 16u) << 24;
       int st = 0, buf = 0;
       unsigned ph = 0, aph = 0;
-      for (int64_t t = unit; t < tiles; t += units) {
+      for (unsigned t = unit; t < tiles; t += units) {
         tc_wait(acc_empty + buf, aph ^ 1, aborted);
         tc_fence_after();
         const uint32_t d = tmem + buf * NT;
@@ -239,80 +275,67 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       }
     }
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    // two warps share a quarter of the lanes, each takes every other chunk
-    constexpr int kChunk = sizeof(TO) == 2 ? 32 : 16;
-    constexpr int kFirst = NT / kChunk >= 2 ? 2 : 1;   // chunks a warp steps over
-    const unsigned stage_out = base + Sh::kStages * Sh::kStage + (warp - 2) * 4096;
-    int buf = 0, ob = 0;
+    const int quad = warp & 3, group = (warp - 2) >> 2;
+    constexpr int kChunk = Sh::kChunk, kTok = MmTile<NT, CG>::kTok;
+    float* ts = (float*)(ring + Sh::kStages * Sh::kStage) + (warp - 2) * Sh::kTok;
+    int buf = 0;
     unsigned aph = 0;
-    for (int64_t t = unit; t < tiles; t += units) {
+    MmTile<NT, CG> next;
+    if ((CG == 2 || S == 1) && unit < tiles) next.load(A, unit, tiles_n, tiles_m, rank, quad, group, lane);
+    for (unsigned t = unit; t < tiles; t += units) {
       if (CG == 1 && S > 1) {
         tc_wait(acc_full + buf, aph, aborted);   // (the cluster finishes below)
         continue;
       }
-      int64_t tn, tm;
-      mm_tile(A, t, tiles_n, tiles_m, &tn, &tm);
-      const int64_t n0 = tn * 128 * CG + (CG == 2 ? 128 * rank : 0) + quad * 32, n = n0 + lane, m0 = tm * NT;
-      const int cols = n0 >= A.N ? 0 : A.M - m0 < NT ? (int)(A.M - m0) : NT;
-      const bool live = n < A.N;
-      const float sw = live ? A.w_scale[n * A.sw] : 0.0f, b = live && A.bias ? A.bias[n * A.sb] : 0.0f;
-      const bool biased = A.bias != nullptr;
-      int c0 = half * kChunk;
-      // lane i holds token c0 + i's scale
-      float ts = lane < kChunk && c0 + lane < cols ? A.a_scale[(m0 + c0 + lane) * A.sa] : 0.0f;
+      // this tile's scales were asked for a tile ago; the next one's are now
+      const MmTile<NT, CG> now = next;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) ts[lane + 32 * i] = now.tok[i];
+      __syncwarp();
+      if (t + units < tiles) next.load(A, t + units, tiles_n, tiles_m, rank, quad, group, lane);
+      const int cols = A.M - now.m0 < NT ? (int)(A.M - now.m0) : NT;
+      const bool live = now.n0 + lane < A.N, biased = A.bias != nullptr;
+      const float sw = now.sw, b = now.b;
       tc_wait(acc_full + buf, aph, aborted);
       tc_fence_after();
+      const uint32_t acc = tmem + buf * NT + ((uint32_t)(quad * 32) << 16);
+      TO* out = (TO*)A.out + now.m0 * A.ldo + now.n0 + lane;
+      uint32_t r[kChunk];
+      int c0 = group * kChunk;
+      if (c0 < cols) mm_ld<kChunk>(acc + c0, r);
 #pragma unroll 1
-      for (; c0 < cols; c0 += kFirst * kChunk) {
-        uint32_t r[kChunk];
-        const uint32_t at = tmem + buf * NT + c0 + ((uint32_t)(quad * 32) << 16);
-        if constexpr (kChunk == 32 && NT < 32) {
-          uint32_t q[16];
-          tmem_ld16(at, q);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = j < 16 ? q[j & 15] : 0;
-        } else if constexpr (kChunk == 32) {
-          tmem_ld32(at, r);
-        } else {
-          tmem_ld16(at, r);
-        }
-        const float now = ts;
-        const int next = c0 + kFirst * kChunk + lane;
-        ts = lane < kChunk && next < cols ? A.a_scale[(m0 + next) * A.sa] : 0.0f;
+      for (int i = 0; c0 < cols; ++i, c0 += 4 * kChunk) {
         tc_wait_ld();
-        if (tma_out) {
-          const unsigned rows = stage_out + ob * 2048;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+        float y[kChunk];
+        const float4* t4 = reinterpret_cast<const float4*>(ts + i * kChunk);
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(__shfl_sync(0xffffffffu, now, j), sw));
-            if (biased) y = __fadd_rn(y, b);
-            if constexpr (sizeof(TO) == 2)
-              asm volatile("st.shared.u16 [%0], %1;\n" ::"r"(rows + j * 64 + lane * 2), "h"(__half_as_ushort(__float2half_rn(y)))
-                           : "memory");
-            else
-              asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(rows + j * 128 + lane * 4), "f"(y) : "memory");
+        for (int j = 0; j < kChunk; j += 4) {
+          const float4 f = t4[j / 4];
+          y[j] = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(f.x, sw));
+          y[j + 1] = __fmul_rn(__int2float_rn((int)r[j + 1]), __fmul_rn(f.y, sw));
+          y[j + 2] = __fmul_rn(__int2float_rn((int)r[j + 2]), __fmul_rn(f.z, sw));
+          y[j + 3] = __fmul_rn(__int2float_rn((int)r[j + 3]), __fmul_rn(f.w, sw));
+        }
+        if (biased) {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) y[j] = __fadd_rn(y[j], b);
+        }
+        // the next chunk's sums are on their way while this one is stored
+        if (c0 + 4 * kChunk < cols) mm_ld<kChunk>(acc + c0 + 4 * kChunk, r);
+        TO* op = out + c0 * A.ldo;
+        if (c0 + kChunk <= cols) {
+          if (live) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j, op += A.ldo) mm_store(op, y[j]);
           }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store2(&map_out, rows, (int)n0, (int)(m0 + c0));
-            bulk_commit();
-          }
-          ob ^= 1;
         } else {
-          TO* op = (TO*)A.out + (m0 + c0) * A.ldo + n;
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            float y = __fmul_rn(__int2float_rn((int)r[j]), __fmul_rn(__shfl_sync(0xffffffffu, now, j), sw));
-            if (biased) y = __fadd_rn(y, b);
-            if (live && c0 + j < cols) mm_store(op, y);
-            op += A.ldo;
-          }
+          for (int j = 0; j < kChunk; ++j, op += A.ldo)
+            if (live && c0 + j < cols) mm_store(op, y[j]);
         }
       }
+      tc_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -321,7 +344,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       }
       if (++buf == 2) buf = 0, aph ^= 1;
     }
-    if (lane == 0) bulk_wait_all();
   }
   __syncwarp();
   if constexpr (CG == 1) {
@@ -333,15 +355,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       cluster_wait();
       tc_fence_after();
       const int per = (NT + S - 1) / S;
-      int64_t tn, tm;
-      mm_tile(A, unit, tiles_n, tiles_m, &tn, &tm);
-      const int64_t m0 = tm * NT;
+      int tn, tm;
+      mm_tile(unit, tiles_n, tiles_m, &tn, &tm);
+      const int64_t m0 = (int64_t)tm * NT;
       const int cols = A.M - m0 < NT ? (int)(A.M - m0) : NT;
       if (warp >= 2) {
         const int quad = warp & 3;
         constexpr int CH = 16;
 #pragma unroll 1
-        for (int c0 = ((warp - 2) >> 2) * CH; c0 < cols; c0 += 2 * CH) {
+        for (int c0 = ((warp - 2) >> 2) * CH; c0 < cols; c0 += 4 * CH) {
           uint32_t r[CH];
           tmem_ld16(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
           tc_wait_ld();
@@ -360,11 +382,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       cluster_wait();
       if (warp >= 2) {
         const int ch = (threadIdx.x - 64) & 127, first = (warp - 2) >> 2;
-        const int64_t n = tn * 128 + ch;
+        const int64_t n = (int64_t)tn * 128 + ch;
         if (n < A.N) {
           const float sw = A.w_scale[n * A.sw], b = A.bias ? A.bias[n * A.sb] : 0.0f;
           const int* red = (const int*)ring;
-          for (int i = first, c = rank + first * S; c < cols; c += 2 * S, i += 2) {
+          for (int i = first, c = rank + first * S; c < cols; c += 4 * S, i += 4) {
             int acc = 0;
             for (int s = 0; s < S; ++s) acc += red[(s * per + i) * 128 + ch];
             float y = __fmul_rn(__int2float_rn(acc), __fmul_rn(A.a_scale[(m0 + c) * A.sa], sw));
@@ -392,7 +414,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
 template <int NT, int CG, typename TO>
 int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   using Sh = MmShape<NT, CG>;
-  CUtensorMap mw, ma, mo = {};
+  CUtensorMap mw, ma;
   const uint64_t dw[2] = {(uint64_t)A.K, (uint64_t)A.N}, da[2] = {(uint64_t)A.K, (uint64_t)A.M};
   const uint64_t sw[1] = {(uint64_t)A.ldw}, sa[1] = {(uint64_t)A.lda};
   const uint32_t bw[2] = {128, 128}, ba[2] = {128, (uint32_t)(NT / CG)};
@@ -400,15 +422,6 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   if ((rc = tma_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.w, dw, sw, bw)) ||
       (rc = tma_map(&ma, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, A.a, da, sa, ba)))
     return rc;
-  const int64_t pitch = A.ldo * (int64_t)sizeof(TO);
-  const int tma_out = S == 1 && ((uintptr_t)A.out & 15) == 0 && (A.M == 1 || (pitch > 0 && pitch % 16 == 0));
-  if (tma_out) {
-    const uint64_t d[2] = {(uint64_t)A.N, (uint64_t)A.M}, st[1] = {(uint64_t)(A.M == 1 ? (A.N + 7) / 8 * 32 : pitch)};
-    const uint32_t box[2] = {32, (uint32_t)(sizeof(TO) == 2 ? (NT < 32 ? NT : 32) : 16)};
-    if ((rc = tma_map(&mo, sizeof(TO) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, A.out, d,
-                      st, box, false)))
-      return rc;
-  }
   auto kern = matmul_tc_kernel<NT, CG, TO>;
   static int raised[64] = {};   // per device: the limit only has to be raised once
   int dev = 0;
@@ -422,7 +435,7 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   const int csize = CG == 2 ? 2 : S;
   const int64_t cap = S > 1 ? tiles : sms / CG;
   const int64_t units = tiles < cap ? tiles : cap;
-  if (units * csize > INT32_MAX) return set_error(BT_ETOOBIG, "%s: too many output values", what);
+  if (tiles + sms > INT32_MAX || units * csize > INT32_MAX) return set_error(BT_ETOOBIG, "%s: too many output values", what);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * csize));
   cfg.blockDim = dim3(kMmThreads);
@@ -433,7 +446,7 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   at[0].val.clusterDim = {(unsigned)csize, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, mo, A, S, tma_out);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mw, ma, A, S);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(BT_ECUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
