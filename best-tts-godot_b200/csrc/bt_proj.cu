@@ -59,6 +59,129 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* x
   }
 }
 
+// Rows on 16-byte boundaries, read once: the TPR threads of a row (a warp, or
+// the CTA) hold it in registers as V 16-byte vectors each, up to
+// TPR * V * 16 bytes; the at most seven values past the last whole vector
+// are one more value on each of the first lanes.  HBM-bound: 32640 rows of
+// 2048 float32 take 48 us of device time, of float16 30 us (82 us for the
+// float32 rows by the kernel above, which reads them twice and serves longer
+// and unaligned rows).
+template <typename T>
+__device__ __forceinline__ void vec_floats(const uint4 v, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = __half22float2(h[i]);
+      f[2 * i] = x.x;
+      f[2 * i + 1] = x.y;
+    }
+  } else {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
+}
+
+// The bits of |v| order like the values, with NaN above infinity, so one
+// integer maximum finds the largest magnitude and keeps a NaN.
+__device__ __forceinline__ unsigned mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// The same for the values of a vector (a NaN anywhere gives a NaN); halves
+// are compared two at a time, as halves.
+template <typename T>
+__device__ __forceinline__ unsigned vec_mag(const uint4 v) {
+  if constexpr (sizeof(T) == 2) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    const float2 f = __half22float2(m);
+    return max(mag_bits(f.x), mag_bits(f.y));
+  } else {
+    return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+  }
+}
+
+__device__ __forceinline__ unsigned q8_sym(float v, float inv) {
+  const float p = __fmul_rn(v, inv);
+  return (unsigned)(p == p ? __float2int_rn(p) : 0) & 0xffu;
+}
+
+template <typename T, int TPR, int V>
+__global__ void __launch_bounds__(256, V <= 8 ? 4 : 2) quantize_rows_vec_kernel(const T* x, int64_t ldx, int64_t rows, int K, int8_t* q,
+                                                                int64_t ldq, float* scale, int64_t lds) {
+  constexpr int N = 16 / sizeof(T), kRows = 256 / TPR;
+  __shared__ unsigned part[8];
+  const int t = threadIdx.x % TPR, nv = K / N, rest = K - nv * N;
+  for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; r < rows; r += (int64_t)gridDim.x * kRows) {
+    const uint4* xv = reinterpret_cast<const uint4*>(x + r * ldx);
+    uint4 v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = t + i * TPR < nv ? __ldcs(xv + t + i * TPR) : make_uint4(0, 0, 0, 0);
+    const float tail = t < rest ? ld1(x + r * ldx, nv * N + t) : 0.0f;
+    unsigned a = max(mag_bits(tail), 0x0d800000u);   // 2^-100
+#pragma unroll
+    for (int i = 0; i < V; ++i) a = max(a, vec_mag<T>(v[i]));
+    a = __reduce_max_sync(0xffffffffu, a);
+    if constexpr (TPR > 32) {
+      __syncthreads();   // (the previous row's reads of part)
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) a = max(a, part[w]);
+    }
+    const float top = __uint_as_float(a > 0x7f800000u ? 0x7fffffffu : a), inv = __fdiv_rn(127.0f, top);
+    if (t == 0) scale[r * lds] = __fdiv_rn(top, 127.0f);
+    int8_t* qr = q + r * ldq;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (t + i * TPR < nv) {
+        float f[N];
+        vec_floats<T>(v[i], f);
+        unsigned w[N / 4];
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j)
+          w[j] = q8_sym(f[4 * j], inv) | q8_sym(f[4 * j + 1], inv) << 8 | q8_sym(f[4 * j + 2], inv) << 16 |
+                 q8_sym(f[4 * j + 3], inv) << 24;
+        if constexpr (N == 4) *reinterpret_cast<unsigned*>(qr + (t + i * TPR) * 4) = w[0];
+        else *reinterpret_cast<uint2*>(qr + (t + i * TPR) * 8) = make_uint2(w[0], w[1]);
+      }
+    if (t < rest) qr[nv * N + t] = (int8_t)q8_sym(tail, inv);
+  }
+}
+
+template <typename T>
+void quantize_run(const T* x, int64_t ldx, int64_t rows, int64_t K, int8_t* q, int64_t ldq, float* scale, int64_t lds,
+                  int sms) {
+  const int64_t row_bytes = K * (int64_t)sizeof(T);
+  const bool one = rows == 1;
+  const int64_t qa = 16 / sizeof(T);   // q is written as 4 or 8 bytes at a time
+  const bool vec = ((uintptr_t)x & 15) == 0 && (one || ldx * (int64_t)sizeof(T) % 16 == 0) && (uintptr_t)q % qa == 0 &&
+                   (one || ldq % qa == 0) && row_bytes <= 256 * 16 * 16;
+  cudaStream_t s = cur_stream();
+  if (!vec) {
+    const int64_t cap = (int64_t)sms * 16;
+    quantize_rows_kernel<T><<<(int)(rows < cap ? rows : cap), kQuantThreads, 0, s>>>(x, ldx, rows, K, q, ldq, scale, lds);
+    return;
+  }
+  // a warp a row where its registers hold the row and there are rows enough
+  // for eight CTAs on every SM; else a CTA a row (510 rows of 2048 float32:
+  // 4.1 us, by warps 5.1 us; 32640 rows: 48 us by warps)
+  const bool warp = row_bytes <= 32 * 16 * 16 && rows > 8 * sms;
+  const int tpr = warp ? 32 : 256, per = (int)((row_bytes + tpr * 16 - 1) / (tpr * 16));
+  const int64_t want = warp ? (rows + 7) / 8 : rows, cap = (int64_t)sms * 8;
+  const int grid = (int)(want < cap ? want : cap);
+  auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(x, ldx, rows, (int)K, q, ldq, scale, lds); };
+  if (warp) {
+    if (per <= 2) go(quantize_rows_vec_kernel<T, 32, 2>);
+    else if (per <= 6) go(quantize_rows_vec_kernel<T, 32, 6>);
+    else if (per <= 8) go(quantize_rows_vec_kernel<T, 32, 8>);
+    else go(quantize_rows_vec_kernel<T, 32, 16>);
+  } else {
+    if (per <= 1) go(quantize_rows_vec_kernel<T, 256, 1>);
+    else if (per <= 4) go(quantize_rows_vec_kernel<T, 256, 4>);
+    else if (per <= 8) go(quantize_rows_vec_kernel<T, 256, 8>);
+    else go(quantize_rows_vec_kernel<T, 256, 16>);
+  }
+}
+
 // ---- int8 product ----------------------------------------------------------
 //   y[m, n] = float(sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n]) (+ bias[n])
 // the sum in int32, exact for K <= 131071 (|a w| <= 2^14).
@@ -547,14 +670,10 @@ extern "C" int bt_quantize_rows(const bt_tensor* x, const bt_tensor* q, const bt
   if (rows == 0) return BT_OK;
   DevInfo di;
   if ((rc = dev_info(&di))) return rc;
-  const int64_t cap = (int64_t)di.sm_count * 16;
-  const int grid = (int)(rows < cap ? rows : cap);
   if (x->dtype == BT_F32)
-    quantize_rows_kernel<float><<<grid, kQuantThreads, 0, cur_stream()>>>((const float*)x->data, ldx, rows, K,
-                                                                          (int8_t*)q->data, ldq, (float*)sp, lds);
+    quantize_run((const float*)x->data, ldx, rows, K, (int8_t*)q->data, ldq, (float*)sp, lds, di.sm_count);
   else
-    quantize_rows_kernel<__half><<<grid, kQuantThreads, 0, cur_stream()>>>((const __half*)x->data, ldx, rows, K,
-                                                                           (int8_t*)q->data, ldq, (float*)sp, lds);
+    quantize_run((const __half*)x->data, ldx, rows, K, (int8_t*)q->data, ldq, (float*)sp, lds, di.sm_count);
   return check_launch(what);
 }
 
