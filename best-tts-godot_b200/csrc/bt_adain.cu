@@ -809,6 +809,7 @@ extern "C" int bt_wait_timeouts(uint32_t* count) {
   unsigned int v = 0;
   cudaError_t e = bt::take_timeouts(&v);
   if (e == cudaSuccess) e = bt::proj_timeouts(&v);
+  if (e == cudaSuccess) e = bt::attn_timeouts(&v);
   if (e != cudaSuccess) return bt::set_error(BT_ECUDA, "bt_wait_timeouts: %s", cudaGetErrorString(e));
   *count = v;
   return BT_OK;

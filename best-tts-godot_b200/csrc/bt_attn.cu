@@ -15,6 +15,8 @@
 #include <stdint.h>
 #include "bt_ops.h"
 #include "bt_internal.h"
+#include "bt_pk.h"
+#include "bt_tc.h"
 
 namespace bt {
 namespace {
@@ -108,7 +110,438 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
   }
 }
 
+
+// ---- float16 on the tensor cores --------------------------------------------
+// A work item is two tiles of 128 queries of one head (256 rows, so that a
+// key tile read once serves both); CTAs walk the items.  Tensor memory holds
+// for each tile the 128 x 128 float32 scores S of the current key tile and the
+// 128 x D output O.
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a query row; reads its
+//                   128 scores, writes the weights P as float16 over them
+//   warp 8          issues S = Q K^T and O += P V (P read from tensor memory)
+//   warp 9          TMA loads: the item's Q tiles, a ring of K and V tiles
+//   warp 10         zeroes the rows of V whose keys take no part (only where
+//                   there are lengths or a mask: a weight of 0 times NaN
+//                   would not be 0)
+// The two tiles take turns: while one's softmax runs, the tensor cores work
+// for the other.
+//
+// Softmax: with c = scale log2(e) and a reference value m per row,
+// p = 2^(s c - m c + 7).  m is the row's running maximum, but it moves (and O
+// and the sum are rescaled) only when the maximum has grown by more than 2^8
+// in p: rescaling O costs a pass over tensor memory, and p <= 2^15 stays in
+// float16's range.  The 2^7 lifts small weights off float16's subnormals: a
+// weight loses precision only below 2^-21 of the reference.  P is rounded to
+// float16 (the tensor cores' operand; relative error 2^-11 a weight, as a
+// float16 result has anyway); the row's sum is of the float32 weights.
+constexpr int kTile = 128;
+constexpr int kAttnThreads = 352;
+constexpr float kGrow = 8.0f, kLift = 7.0f;
+
+struct AttnTc {
+  AttnArgs a;
+  int32_t q_mul[2], k_mul[2], v_mul[2];   // 0 where an axis (head, batch) is broadcast
+  int32_t q_tiles;                        // items of a head
+  uint32_t items;
+  int32_t wide;                           // out's rows: 32-, 16- or 2-byte stores
+};
+
+template <int DP>
+struct AttnShape {
+  static constexpr int kPanel = kTile * 128;               // 128 rows of 64 values
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kRows = kPanel * kPanels;           // one tile of Q, K or V
+  static constexpr int kSlots = DP == 64 ? 8 : 4;          // ring of K and V tiles
+  static constexpr int kSmem = 1024 + (2 + kSlots) * kRows + 512;
+};
+
+// The valid keys of a key tile as four words; all ones where every key is.
+__device__ __forceinline__ unsigned tail_word(int left, int i) {   // keys left from the tile's start
+  const int n = left - 32 * i;
+  return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// The scores of keys that take no part become -inf.
+__device__ __forceinline__ void only(uint32_t (&s)[32], unsigned w) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j] = w >> j & 1 ? s[j] : 0xff800000u;
+}
+
+struct ItemPos {
+  int64_t b;
+  int h, t0;
+};
+__device__ __forceinline__ ItemPos item_pos(const AttnTc& A, uint32_t it) {
+  const uint32_t head = it / (uint32_t)A.q_tiles;
+  ItemPos p;
+  p.t0 = (int)(it - head * (uint32_t)A.q_tiles) * 2 * kTile;
+  p.b = head / (uint32_t)A.a.H;
+  p.h = (int)(head - (uint32_t)p.b * (uint32_t)A.a.H);
+  return p;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnTc A) {
+  using Sh = AttnShape<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  const unsigned base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const unsigned ring = base + 2 * Sh::kRows;
+  uint64_t* bars = (uint64_t*)(smem + (2 + Sh::kSlots) * Sh::kRows);
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8;
+  uint64_t *kv_full = bars + 10, *kv_empty = kv_full + Sh::kSlots, *v_ok = kv_empty + Sh::kSlots;
+  uint32_t* slot = (uint32_t*)(v_ok + Sh::kSlots);
+  volatile int* aborted = (volatile int*)(slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const AttnArgs& a = A.a;
+  const bool fix_v = a.lengths || a.mask;
+  if (threadIdx.x == 0) {
+    *aborted = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_full + i, 1);
+    }
+    for (int i = 0; i < Sh::kSlots; ++i) {
+      mbar_init(kv_full + i, 1);
+      mbar_init(kv_empty + i, 1);
+      mbar_init(v_ok + i, 1);
+    }
+    tma_prefetch(&map_q);
+    tma_prefetch(&map_k);
+    tma_prefetch(&map_v);
+  }
+  if (warp == 8) tmem_alloc<1>(slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+
+  if (warp < 8) {
+    const int tile = warp >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t sp = tmem + tile * kTile + lanes, op = tmem + 256 + tile * DP + lanes;
+    const float c = a.scale * 1.4426950408889634f;   // log2(e)
+    unsigned s_ph = 0, o_ph = 0;
+    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
+      const ItemPos pos = item_pos(A, it);
+      const int64_t t = pos.t0 + tile * kTile + (warp & 3) * 32 + lane;
+      if (pos.t0 + tile * kTile >= a.Tq) continue;
+      const int n = (int)keys_of(a, pos.b);
+      const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
+      float m = -INFINITY, mc = 0.0f;   // the reference (-inf: no key yet) and m c - 7
+      float2 l = {0.0f, 0.0f};
+      uint8_t mb[4] = {1, 1, 1, 1};
+      if (mask)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mb[i] = 32 * i + lane < n ? mask[(int64_t)(32 * i + lane) * a.mask_sk] : 0;
+      for (int k0 = 0; k0 < n; k0 += kTile) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = tail_word(n - k0, i);
+        if (mask) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = __ballot_sync(0xffffffffu, mb[i] != 0);
+          // the next tile's bytes, while this one is computed
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int k = k0 + kTile + 32 * i + lane;
+            mb[i] = k < n ? mask[(int64_t)k * a.mask_sk] : 0;
+          }
+        }
+        tc_wait(s_full + tile, s_ph, aborted);
+        s_ph ^= 1;
+        tc_fence_after();
+        const bool part = (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
+        uint32_t s[2][32];
+        float mx[2] = {-INFINITY, -INFINITY};
+        tmem_ld32(sp, s[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t(&x)[32] = s[i & 1];
+          tc_wait_ld();
+          if (i < 3) tmem_ld32(sp + 32 * (i + 1), s[(i + 1) & 1]);
+          if (part) only(x, w[i]);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
+            mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])));
+          }
+        }
+        const float top = fmaxf(mx[0], mx[1]);
+        const bool grow = top > m && (m == -INFINITY || (top - m) * c > kGrow);
+        if (__any_sync(0xffffffffu, grow)) {
+          // exp2(-inf) = 0 where there was no key before: O and l are 0 then
+          // or, in the first tile, not yet written
+          const float keep = grow ? (m == -INFINITY ? 0.0f : exp2f((m - top) * c)) : 1.0f;
+          if (grow) {
+            m = top;
+            mc = fmaf(top, c, -kLift);
+            l.x *= keep;
+            l.y *= keep;
+          }
+          if (k0 > 0) {
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+              uint32_t o[32];
+              tmem_ld32(op + 32 * i, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+              tmem_st32(op + 32 * i, o);
+            }
+          }
+        }
+        // the scores again (keeping all 128 beside the rescaling above would
+        // not fit the registers), 32 at a time, the next 32 on their way
+        const float2 c2 = {c, c}, mc2 = {-mc, -mc};
+        float2 part_l[4] = {};
+        tmem_ld32(sp, s[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t(&x)[32] = s[i & 1];
+          tc_wait_ld();
+          if (i < 3) tmem_ld32(sp + 32 * (i + 1), s[(i + 1) & 1]);
+          if (part) only(x, w[i]);
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float2 e = pk_fma(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, mc2);
+            asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+            asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+            part_l[j & 3] = pk_add(part_l[j & 3], e);
+            const __half2 h = __float22half2_rn(e);
+            p[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          // P's column j holds keys 2 j and 2 j + 1: 32 scores become 16
+          // columns, behind the scores still to be read
+          tmem_st16(sp + 16 * i, p);
+        }
+        l = pk_add(l, pk_add(pk_add(part_l[0], part_l[1]), pk_add(part_l[2], part_l[3])));
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + tile);
+      }
+      // the result: O / l
+      const float sum = l.x + l.y;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      __half* out = (__half*)a.out + pos.b * a.os[0] + pos.h * a.os[1] + t * a.os[2];
+      if (n > 0) {
+        tc_wait(o_full + tile, o_ph, aborted);
+        o_ph ^= 1;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        if (32 * i >= a.D) break;
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_ld32(op + 32 * i, o);
+          tc_wait_ld();
+        }
+        uint32_t y[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          // (the select keeps a row without keys 0 whatever O holds)
+          const __half2 h = sum == 0.0f ? __floats2half2_rn(0.0f, 0.0f)
+                                        : __floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
+          y[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (t < a.Tq) {
+          const int left = a.D - 32 * i;
+          if (A.wide == 16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (8 * j < left)
+                *reinterpret_cast<uint4*>(out + 32 * i + 8 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+          } else {
+            const __half* e = reinterpret_cast<const __half*>(y);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j < left) out[(int64_t)(32 * i + j) * a.os[3]] = e[j];
+          }
+        }
+      }
+      tc_fence_before();   // (O is read before this warp's next arrival lets it be written)
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      constexpr uint32_t id_s = 1u << 4 | (kTile / 8u) << 17 | (kTile / 16u) << 24;
+      constexpr uint32_t id_o = 1u << 4 | 1u << 16 | (DP / 8u) << 17 | (kTile / 16u) << 24;   // V: rows along the sum
+      unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
+      uint32_t g = 0;   // K and V tiles used so far: K of block j of an item is tile g + 2 j, V the one after
+      auto at = [&](uint32_t x) { return ring + x % Sh::kSlots * Sh::kRows; };
+      auto ph = [&](uint32_t x) { return x / Sh::kSlots & 1; };
+      for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
+        const ItemPos pos = item_pos(A, it);
+        const int nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
+        if (nb == 0) continue;
+        const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1;
+        for (int j = 0; j <= nb; ++j) {
+          const uint32_t k = g + 2 * j, v = k - 1;
+          if (j < nb) tc_wait(kv_full + k % Sh::kSlots, ph(k), aborted);
+          if (j > 0) tc_wait((fix_v ? v_ok : kv_full) + v % Sh::kSlots, ph(v), aborted);
+          for (int i = 0; i < tiles; ++i) {
+            if (j > 0) {
+              tc_wait(p_full + i, p_ph[i], aborted);
+              p_ph[i] ^= 1;
+              tc_fence_after();
+              const uint64_t dv = smem_desc(at(v), Sh::kPanel, 1024);
+#pragma unroll
+              for (int x = 0; x < kTile / 16; ++x)
+                mma_f16_ts(tmem + 256 + i * DP, tmem + i * kTile + 8 * x, dv + 128 * x, id_o, j > 1 || x > 0);
+              if (j == nb) mma_commit(o_full + i);
+            }
+            if (j < nb) {
+              if (j == 0) {
+                tc_wait(q_full + i, q_ph[i], aborted);
+                q_ph[i] ^= 1;
+              }
+              tc_fence_after();
+              // (a descriptor's low bits are the address / 16)
+              const uint64_t dq = smem_desc(base + i * Sh::kRows, 16, 1024), dk = smem_desc(at(k), 16, 1024);
+#pragma unroll
+              for (int x = 0; x < DP / 16; ++x) {
+                constexpr int kStep = Sh::kPanel / 16;
+                mma_f16_ss(tmem + i * kTile, dq + (x / 4 * kStep + x % 4 * 2), dk + (x / 4 * kStep + x % 4 * 2), id_s, x > 0);
+              }
+              mma_commit(s_full + i);
+              if (j == nb - 1) mma_commit(q_empty + i);
+            }
+          }
+          if (j > 0) mma_commit(kv_empty + v % Sh::kSlots);
+          if (j < nb) mma_commit(kv_empty + k % Sh::kSlots);
+        }
+        g += 2 * nb;
+      }
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      unsigned q_ph[2] = {1, 1};
+      uint32_t g = 0;
+      for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
+        const ItemPos pos = item_pos(A, it);
+        const int nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
+        if (nb == 0) continue;
+        const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1, b = (int)pos.b, hk = pos.h / (int)a.G;
+        auto load = [&](const CUtensorMap* m, unsigned dst, uint64_t* bar, int t0, int h, int bb) {
+          mbar_arrive_expect_tx(bar, Sh::kRows);
+#pragma unroll
+          for (int x = 0; x < Sh::kPanels; ++x) tma_load4(dst + x * Sh::kPanel, m, smem_u32(bar), 64 * x, t0, h, bb);
+        };
+        for (int i = 0; i < tiles; ++i) {
+          tc_wait(q_empty + i, q_ph[i], aborted);
+          q_ph[i] ^= 1;
+          load(&map_q, base + i * Sh::kRows, q_full + i, pos.t0 + i * kTile, pos.h * A.q_mul[0], b * A.q_mul[1]);
+        }
+        for (int j = 0; j < nb; ++j) {
+          for (int y = 0; y < 2; ++y, ++g) {
+            const int sl = (int)(g % Sh::kSlots);
+            tc_wait(kv_empty + sl, (g / Sh::kSlots & 1) ^ 1, aborted);
+            load(y ? &map_v : &map_k, ring + sl * Sh::kRows, kv_full + sl, j * kTile, hk * (y ? A.v_mul : A.k_mul)[0],
+                 b * (y ? A.v_mul : A.k_mul)[1]);
+          }
+        }
+      }
+      for (int i = 0; i < Sh::kSlots; ++i, ++g)   // every tile used: no arrival is under way when the CTA ends
+        tc_wait(kv_empty + g % Sh::kSlots, (g / Sh::kSlots & 1) ^ 1, aborted);
+      for (int i = 0; i < 2; ++i) tc_wait(q_empty + i, q_ph[i], aborted);
+    }
+  } else if (warp == 10 && fix_v) {
+    uint32_t g = 1;
+    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
+      const ItemPos pos = item_pos(A, it);
+      const int n = (int)keys_of(a, pos.b);
+      const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
+      for (int k0 = 0; k0 < n; k0 += kTile, g += 2) {
+        bool in[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = k0 + 32 * i + lane;
+          in[i] = k < n && (!mask || mask[(int64_t)k * a.mask_sk]);
+        }
+        const int sl = (int)(g % Sh::kSlots);
+        tc_wait(kv_full + sl, g / Sh::kSlots & 1, aborted);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          unsigned out = ~__ballot_sync(0xffffffffu, in[i]);
+          any |= out != 0;
+          // eight lanes clear a 128-byte row, four rows at a time
+          for (; out; ) {
+            unsigned pick = out;   // the (lane / 8)-th of the rows still to clear
+            for (int y = 0; y < (lane >> 3); ++y) pick &= pick - 1;
+            if (pick) {
+              const int row = 32 * i + __ffs(pick) - 1;
+#pragma unroll
+              for (int x = 0; x < Sh::kPanels; ++x)
+                *reinterpret_cast<uint4*>(smem + (2 + sl) * Sh::kRows + x * Sh::kPanel + row * 128 + (lane & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+            }
+            for (int y = 0; y < 4; ++y) out &= out - 1;
+          }
+        }
+        if (any) fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_ok + sl);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*aborted) {   // copies may still be in flight: give them time to land
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) {}
+  }
+  if (warp == 8) tmem_free<1>(tmem, 512);
+}
+
+// A tensor map over [B, H, T, D] (innermost D), 64 x 128 boxes; false where
+// the strides or the base do not suit one.  mul: 0 for a broadcast head or
+// batch axis, whose extent in the map is 1.
+bool attn_map(CUtensorMap* m, const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, int64_t D, int32_t* mul,
+              int* rc) {
+  *rc = BT_OK;
+  if (((uintptr_t)p & 15) || (D > 1 && st[3] != 1) || T < 1) return false;
+  const int64_t ext[3] = {T, H, B}, str[3] = {st[2], st[1], st[0]};
+  uint64_t dims[4] = {(uint64_t)D, 1, 1, 1}, bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    bytes[i] = (uint64_t)(D * 2 + 15) / 16 * 16;
+    if (i) mul[i - 1] = 0;
+    if (ext[i] == 1) continue;
+    if (str[i] == 0 && i) continue;
+    if (str[i] <= 0 || str[i] % 8 || str[i] >= (int64_t)1 << 38) return false;
+    dims[i + 1] = (uint64_t)ext[i];
+    bytes[i] = (uint64_t)str[i] * 2;
+    if (i) mul[i - 1] = 1;
+  }
+  const uint32_t box[4] = {64, kTile, 1, 1};
+  *rc = tma_map(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p, dims, bytes, box);
+  return *rc == BT_OK;
+}
+
+template <int DP>
+int attn_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnTc& A, int sms) {
+  auto kern = attn_tc_kernel<DP>;
+  constexpr int smem = AttnShape<DP>::kSmem;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  const int grid = (int)(A.items < (uint32_t)sms ? A.items : (uint32_t)sms);
+  kern<<<grid, kAttnThreads, smem, cur_stream()>>>(mq, mk, mv, A);
+  return check_launch("bt_attention");
+}
+
 }  // namespace
+
+cudaError_t attn_timeouts(unsigned int* sum) { return take_timeouts(sum); }
+
 }  // namespace bt
 
 using namespace bt;
@@ -175,6 +608,22 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   A.out = out->data;
   DevInfo di;
   if ((rc = dev_info(&di))) return rc;
+  if (q->dtype == BT_F16 && A.Tk > 0 && A.Tq > 16) {
+    AttnTc P{};
+    CUtensorMap mq, mk, mv;
+    const int64_t q_tiles = (A.Tq + 2 * kTile - 1) / (2 * kTile), items = A.B * A.H * q_tiles;
+    if (items < INT32_MAX && attn_map(&mq, A.q, A.qs, A.B, A.H, A.Tq, D, P.q_mul, &rc) &&
+        attn_map(&mk, A.k, A.ks, A.B, Hk, A.Tk, D, P.k_mul, &rc) && attn_map(&mv, A.v, A.vs, A.B, Hk, A.Tk, D, P.v_mul, &rc)) {
+      P.a = A;
+      P.q_tiles = (int32_t)q_tiles;
+      P.items = (uint32_t)items;
+      const bool rows16 = ((uintptr_t)A.out & 15) == 0 && D % 8 == 0 && A.os[3] == 1 && A.os[0] % 8 == 0 && A.os[1] % 8 == 0 &&
+                          A.os[2] % 8 == 0;
+      P.wide = rows16 ? 16 : 2;
+      return D <= 64 ? attn_tc_launch<64>(mq, mk, mv, P, di.sm_count) : attn_tc_launch<128>(mq, mk, mv, P, di.sm_count);
+    }
+    if (rc) return rc;
+  }
   const int64_t want = (rows + kRowWarps - 1) / kRowWarps, cap = (int64_t)di.sm_count * 16;
   const int grid = (int)(want < cap ? want : cap);
   if (q->dtype == BT_F32) attn_rows_kernel<float><<<grid, 32 * kRowWarps, 0, cur_stream()>>>(A, rows);

@@ -58,8 +58,9 @@ int adain_v3(const bt_adain_args* p, uint32_t* const* range = nullptr);
 // current stream.
 int dq_range_launch(const void* x, int32_t dtype, int64_t n, uint32_t* rec);
 
-// The bounded waits that gave up in the kernels of bt_proj.cu: added to *sum
-// and reset (see bt_wait_timeouts).
+// The bounded waits that gave up in the kernels of bt_proj.cu / bt_attn.cu:
+// added to *sum and reset (see bt_wait_timeouts).
 cudaError_t proj_timeouts(unsigned int* sum);
+cudaError_t attn_timeouts(unsigned int* sum);
 
 }  // namespace bt

@@ -255,8 +255,8 @@ int bt_adain_snake(const bt_adain_args* a);
  *           Snake output) for each quantised conv input. */
 int bt_adain_snake_range(const bt_adain_args* a, uint32_t* range);
 /* The number of bounded waits on copies and matrix instructions in the
- * bt_adain_snake / bt_adain_snake_range and bt_matmul_int8 kernels that gave
- * up since the last call (each such
+ * bt_adain_snake / bt_adain_snake_range, bt_matmul_int8 and bt_attention
+ * kernels that gave up since the last call (each such
  * wait records itself and lets its kernel run on with unfinished data, so a
  * copy that never lands cannot hang the GPU); the count is then reset.
  * Synchronous (waits for the device).  *count == 0 after a run means every
