@@ -114,17 +114,21 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // ---- float16 on the tensor cores --------------------------------------------
 // A work item is two tiles of 128 queries of one head (256 rows, so that a
 // key tile read once serves both); CTAs walk the items.  Tensor memory holds
-// for each tile the 128 x 128 float32 scores S of the current key tile and the
-// 128 x D output O.
-//   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a query row; reads its
-//                   128 scores, writes the weights P as float16 over them
+// for each tile the 128 x 128 float32 scores S of the current key tile, the
+// float16 weights P (D <= 64: beside S; else over S) and the 128 x D output O.
+//   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a query row, reads its
+//                   128 scores into registers, writes its weights
 //   warp 8          issues S = Q K^T and O += P V (P read from tensor memory)
 //   warp 9          TMA loads: the item's Q tiles, a ring of K and V tiles
 //   warp 10         zeroes the rows of V whose keys take no part (only where
 //                   there are lengths or a mask: a weight of 0 times NaN
 //                   would not be 0)
 // The two tiles take turns: while one's softmax runs, the tensor cores work
-// for the other.
+// for the other; with P beside S the next scores are also computed while the
+// softmax still works on these.  (Blocks of 64 keys with two score buffers a
+// tile measured slower, 655 against 536 us at 16 heads of 8192 x 8192 x 64:
+// the softmax is bound by its instructions' latencies, and each block has a
+// fixed part of about 700 clocks.)
 //
 // Softmax: with c = scale log2(e) and a reference value m per row,
 // p = 2^(s c - m c + 7).  m is the row's running maximum, but it moves (and O
@@ -135,8 +139,9 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // float16 (the tensor cores' operand; relative error 2^-11 a weight, as a
 // float16 result has anyway); the row's sum is of the float32 weights.
 constexpr int kTile = 128;
-constexpr int kAttnThreads = 352;
+constexpr int kAttnThreads = 384;
 constexpr float kGrow = 8.0f, kLift = 7.0f;
+constexpr int kPolyOf8 = 2;   // of eight pairs of weights, those on the FMA pipe
 
 struct AttnTc {
   AttnArgs a;
@@ -152,6 +157,10 @@ struct AttnShape {
   static constexpr int kPanels = DP / 64;
   static constexpr int kRows = kPanel * kPanels;           // one tile of Q, K or V
   static constexpr int kSlots = DP == 64 ? 8 : 4;          // ring of K and V tiles
+  static constexpr bool kBeside = DP == 64;                // P beside S
+  static constexpr int kP = kBeside ? 256 : 0;             // tensor memory: S at 0, 128
+  static constexpr int kPStep = kBeside ? 64 : 128;
+  static constexpr int kO = kBeside ? 384 : 256;
   static constexpr int kSmem = 1024 + (2 + kSlots) * kRows + 512;
 };
 
@@ -165,6 +174,31 @@ __device__ __forceinline__ unsigned tail_word(int left, int i) {   // keys left 
 __device__ __forceinline__ void only(uint32_t (&s)[32], unsigned w) {
 #pragma unroll
   for (int j = 0; j < 32; ++j) s[j] = w >> j & 1 ? s[j] : 0xff800000u;
+}
+
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values on the FMA pipe (the special-function unit gives four
+// exponentials a clock and scheduler, and bounds this softmax): x = n + f with
+// n = rint(x) from the sum with 1.5 2^23, 2^f by a polynomial of degree 4 on
+// [-1/2, 1/2] (minimax by exchange, relative error 2.6e-6), n added to the
+// exponent.  x <= 16; below -126 gives 2^-126.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 t = pk_add(x, pk(12582912.0f));
+  const float2 f = pk_fma(pk_add(t, pk(-12582912.0f)), pk(-1.0f), x);
+  float2 p = pk_fma(pk(0.009570101911165427f), f, pk(0.055917860319388245f));
+  p = pk_fma(p, f, pk(0.2402474482786378f));
+  p = pk_fma(p, f, pk(0.6931218147366892f));
+  p = pk_fma(p, f, pk(0.9999992614457122f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 struct ItemPos {
@@ -190,8 +224,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const unsigned ring = base + 2 * Sh::kRows;
   uint64_t* bars = (uint64_t*)(smem + (2 + Sh::kSlots) * Sh::kRows);
-  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8;
-  uint64_t *kv_full = bars + 10, *kv_empty = kv_full + Sh::kSlots, *v_ok = kv_empty + Sh::kSlots;
+  uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 6, *p_full = bars + 8;
+  uint64_t* pv_done = bars + 10;   // [tile][key tile's parity]: two, so that a phase may pass unwaited for
+  uint64_t *kv_full = bars + 14, *kv_empty = kv_full + Sh::kSlots, *v_ok = kv_empty + Sh::kSlots;
   uint32_t* slot = (uint32_t*)(v_ok + Sh::kSlots);
   volatile int* aborted = (volatile int*)(slot + 1);
 
@@ -203,9 +238,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
+      mbar_init(pv_done + 2 * i, 1);
+      mbar_init(pv_done + 2 * i + 1, 1);
       mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 4);
       mbar_init(p_full + i, 4);
-      mbar_init(o_full + i, 1);
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
       mbar_init(kv_full + i, 1);
@@ -225,9 +262,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if (warp < 8) {
     const int tile = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t sp = tmem + tile * kTile + lanes, op = tmem + 256 + tile * DP + lanes;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");   // 256 x 208 + 128 x 88 = 384 x 168
+    const uint32_t sp = tmem + tile * kTile + lanes, pp = tmem + Sh::kP + tile * Sh::kPStep + lanes;
+    const uint32_t op = tmem + Sh::kO + tile * DP + lanes;
     const float c = a.scale * 1.4426950408889634f;   // log2(e)
-    unsigned s_ph = 0, o_ph = 0;
+    uint32_t g = 0;   // key tiles this query tile has worked on
     for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
       const ItemPos pos = item_pos(A, it);
       const int64_t t = pos.t0 + tile * kTile + (warp & 3) * 32 + lane;
@@ -240,44 +279,51 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (mask)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mb[i] = 32 * i + lane < n ? mask[(int64_t)(32 * i + lane) * a.mask_sk] : 0;
-      for (int k0 = 0; k0 < n; k0 += kTile) {
-        unsigned w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = tail_word(n - k0, i);
+      for (int k0 = 0; k0 < n; k0 += kTile, ++g) {
+        unsigned w[4] = {~0u, ~0u, ~0u, ~0u};
+        bool part = n - k0 < kTile;
         if (mask) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = __ballot_sync(0xffffffffu, mb[i] != 0);
+          part = (w[0] & w[1] & w[2] & w[3]) != ~0u;
           // the next tile's bytes, while this one is computed
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int k = k0 + kTile + 32 * i + lane;
             mb[i] = k < n ? mask[(int64_t)k * a.mask_sk] : 0;
           }
+        } else if (part) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = tail_word(n - k0, i);
         }
-        tc_wait(s_full + tile, s_ph, aborted);
-        s_ph ^= 1;
+        tc_wait(s_full + tile, g & 1, aborted);
         tc_fence_after();
-        const bool part = (w[0] & w[1] & w[2] & w[3]) != 0xffffffffu;
-        uint32_t s[2][32];
-        float mx[2] = {-INFINITY, -INFINITY};
-        tmem_ld32(sp, s[0]);
+        uint32_t s[4][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t(&x)[32] = s[i & 1];
-          tc_wait_ld();
-          if (i < 3) tmem_ld32(sp + 32 * (i + 1), s[(i + 1) & 1]);
-          if (part) only(x, w[i]);
+        for (int i = 0; i < 4; ++i) tmem_ld32(sp + 32 * i, s[i]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
-            mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])));
-          }
+        for (int i = 0; i < 4; ++i) tc_loaded(s[i]);
+        if constexpr (Sh::kBeside) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free + tile);
         }
-        const float top = fmaxf(mx[0], mx[1]);
-        const bool grow = top > m && (m == -INFINITY || (top - m) * c > kGrow);
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) only(s[i], w[i]);
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1]));
+        float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
+        // a NaN among the scores, or +inf (inf - inf), makes the row NaN by
+        // way of its reference; the comparisons below are true for NaN
+        const bool grow = !(top <= m) && (m == -INFINITY || !((top - m) * c <= kGrow));
         if (__any_sync(0xffffffffu, grow)) {
-          // exp2(-inf) = 0 where there was no key before: O and l are 0 then
-          // or, in the first tile, not yet written
+          if (top == INFINITY) top = NAN;
+          // where there was no key before, O and l are 0 or not yet written
           const float keep = grow ? (m == -INFINITY ? 0.0f : exp2f((m - top) * c)) : 1.0f;
           if (grow) {
             m = top;
@@ -286,41 +332,41 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             l.y *= keep;
           }
           if (k0 > 0) {
+            tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);   // O holds every key tile before
+            tc_fence_after();
+            // (a few columns at a time: the 128 scores stay in registers)
+#pragma unroll 1
+            for (int i = 0; i < DP; i += 16) {
+              uint32_t o[16];
+              tmem_ld16(op + i, o);
+              tc_loaded(o);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-              uint32_t o[32];
-              tmem_ld32(op + 32 * i, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-              tmem_st32(op + 32 * i, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+              tmem_st16(op + i, o);
             }
           }
         }
-        // the scores again (keeping all 128 beside the rescaling above would
-        // not fit the registers), 32 at a time, the next 32 on their way
         const float2 c2 = {c, c}, mc2 = {-mc, -mc};
         float2 part_l[4] = {};
-        tmem_ld32(sp, s[0]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t(&x)[32] = s[i & 1];
-          tc_wait_ld();
-          if (i < 3) tmem_ld32(sp + 32 * (i + 1), s[(i + 1) & 1]);
-          if (part) only(x, w[i]);
           uint32_t p[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            float2 e = pk_fma(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, mc2);
-            asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
-            asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+            float2 e = pk_fma(make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1])), c2, mc2);
+            if (j % 8 >= 8 - kPolyOf8) {
+              e = exp2_poly(e);
+            } else {
+              asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+              asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+            }
             part_l[j & 3] = pk_add(part_l[j & 3], e);
             const __half2 h = __float22half2_rn(e);
             p[j] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          // P's column j holds keys 2 j and 2 j + 1: 32 scores become 16
-          // columns, behind the scores still to be read
-          tmem_st16(sp + 16 * i, p);
+          // (P beside S: the last product has read its weights by now)
+          if (Sh::kBeside && i == 0 && k0 > 0) tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);
+          tmem_st16(pp + 16 * i, p);   // column j: keys 2 j and 2 j + 1
         }
         l = pk_add(l, pk_add(pk_add(part_l[0], part_l[1]), pk_add(part_l[2], part_l[3])));
         tc_wait_st();
@@ -330,11 +376,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       // the result: O / l
       const float sum = l.x + l.y;
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      // (a row with a key has a weight of at least 2^-1)
+      const bool none = sum < 0x1p-60f;
+      const float inv = 1.0f / sum;
       __half* out = (__half*)a.out + pos.b * a.os[0] + pos.h * a.os[1] + t * a.os[2];
       if (n > 0) {
-        tc_wait(o_full + tile, o_ph, aborted);
-        o_ph ^= 1;
+        // (s_full of the last key tile came after the product two before it,
+        // so only the last two are open, one on each barrier)
+        tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);
         tc_fence_after();
       }
 #pragma unroll
@@ -343,13 +392,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         uint32_t o[32];
         if (n > 0) {
           tmem_ld32(op + 32 * i, o);
-          tc_wait_ld();
+          tc_loaded(o);
         }
         uint32_t y[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           // (the select keeps a row without keys 0 whatever O holds)
-          const __half2 h = sum == 0.0f ? __floats2half2_rn(0.0f, 0.0f)
+          const __half2 h = none ? __floats2half2_rn(0.0f, 0.0f)
                                         : __floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
           y[j] = *reinterpret_cast<const uint32_t*>(&h);
         }
@@ -370,55 +419,97 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       tc_fence_before();   // (O is read before this warp's next arrival lets it be written)
     }
-  } else if (warp == 8) {
-    if (lane == 0) {
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+  }
+  if (warp == 8) {
+    // The whole warp walks the loop and one elected lane issues: the operands
+    // are then known to be uniform (with the loop on one lane, issuing the
+    // sixteen products of a step took 3300 clocks).
+    {
       constexpr uint32_t id_s = 1u << 4 | (kTile / 8u) << 17 | (kTile / 16u) << 24;
       constexpr uint32_t id_o = 1u << 4 | 1u << 16 | (DP / 8u) << 17 | (kTile / 16u) << 24;   // V: rows along the sum
-      unsigned q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-      uint32_t g = 0;   // K and V tiles used so far: K of block j of an item is tile g + 2 j, V the one after
-      auto at = [&](uint32_t x) { return ring + x % Sh::kSlots * Sh::kRows; };
-      auto ph = [&](uint32_t x) { return x / Sh::kSlots & 1; };
-      for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
-        const ItemPos pos = item_pos(A, it);
-        const int nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
-        if (nb == 0) continue;
-        const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1;
-        for (int j = 0; j <= nb; ++j) {
-          const uint32_t k = g + 2 * j, v = k - 1;
-          if (j < nb) tc_wait(kv_full + k % Sh::kSlots, ph(k), aborted);
-          if (j > 0) tc_wait((fix_v ? v_ok : kv_full) + v % Sh::kSlots, ph(v), aborted);
-          for (int i = 0; i < tiles; ++i) {
-            if (j > 0) {
-              tc_wait(p_full + i, p_ph[i], aborted);
-              p_ph[i] ^= 1;
-              tc_fence_after();
-              const uint64_t dv = smem_desc(at(v), Sh::kPanel, 1024);
+      unsigned q_ph[2] = {0, 0};
+      uint32_t g[2] = {0, 0};   // key tiles scored so far, for each query tile
+      uint32_t r = 0;           // K and V tiles used so far: K tile j of an item is r + 2 j, its V the one after
+      // an item's key and query tiles; the next item with keys from `it` on
+      uint32_t it = blockIdx.x;
+      int nb = 0, tiles = 0;
+      auto seek = [&]() {
+        for (; it < A.items; it += gridDim.x) {
+          const ItemPos pos = item_pos(A, it);
+          nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
+          tiles = pos.t0 + kTile < a.Tq ? 2 : 1;
+          if (nb > 0) return true;
+        }
+        return false;
+      };
+      // S of query tile i and K tile kt
+      auto score = [&](int i, uint32_t kt, bool first, bool last) {
+        if (first) {
+          tc_wait(q_full + i, q_ph[i], aborted);
+          q_ph[i] ^= 1;
+        }
+        tc_wait(kv_full + kt % Sh::kSlots, kt / Sh::kSlots & 1, aborted);
+        if (Sh::kBeside && g[i] > 0) tc_wait(s_free + i, (g[i] - 1) & 1, aborted);
+        tc_fence_after();
+        // (a descriptor's low bits are the address / 16)
+        const uint64_t dq = smem_desc(base + i * Sh::kRows, 16, 1024), dk = smem_desc(ring + kt % Sh::kSlots * Sh::kRows, 16, 1024);
+        if (elect_one()) {
+#pragma unroll
+          for (int x = 0; x < DP / 16; ++x) {
+            constexpr int kStep = Sh::kPanel / 16;
+            mma_f16_ss(tmem + i * kTile, dq + (x / 4 * kStep + x % 4 * 2), dk + (x / 4 * kStep + x % 4 * 2), id_s, x > 0);
+          }
+          mma_commit(s_full + i);
+          if (last) mma_commit(q_empty + i);
+        }
+        __syncwarp();
+        ++g[i];
+      };
+      auto free_kv = [&](uint32_t x) {
+        if (elect_one()) mma_commit(kv_empty + x % Sh::kSlots);
+        __syncwarp();
+      };
+      bool more = seek();
+      if (more) {
+        for (int i = 0; i < tiles; ++i) score(i, r, true, nb == 1);
+        free_kv(r);
+      }
+      while (more) {
+        const int nb0 = nb, tiles0 = tiles;
+        for (int j = 0; j < nb0; ++j) {
+          const bool last = j == nb0 - 1;
+          const uint32_t vt = r + 2 * j + 1, kt = vt + 1;
+          if (Sh::kBeside && !last) {
+            for (int i = 0; i < tiles0; ++i) score(i, kt, false, j + 1 == nb0 - 1);
+            free_kv(kt);
+          }
+          tc_wait((fix_v ? v_ok : kv_full) + vt % Sh::kSlots, vt / Sh::kSlots & 1, aborted);
+          for (int i = 0; i < tiles0; ++i) {
+            const uint32_t b = Sh::kBeside && !last ? g[i] - 2 : g[i] - 1;
+            tc_wait(p_full + i, b & 1, aborted);
+            tc_fence_after();
+            const uint64_t dv = smem_desc(ring + vt % Sh::kSlots * Sh::kRows, Sh::kPanel, 1024);
+            if (elect_one()) {
 #pragma unroll
               for (int x = 0; x < kTile / 16; ++x)
-                mma_f16_ts(tmem + 256 + i * DP, tmem + i * kTile + 8 * x, dv + 128 * x, id_o, j > 1 || x > 0);
-              if (j == nb) mma_commit(o_full + i);
+                mma_f16_ts(tmem + Sh::kO + i * DP, tmem + Sh::kP + i * Sh::kPStep + 8 * x, dv + 128 * x, id_o, j > 0 || x > 0);
+              mma_commit(pv_done + 2 * i + (b & 1));
             }
-            if (j < nb) {
-              if (j == 0) {
-                tc_wait(q_full + i, q_ph[i], aborted);
-                q_ph[i] ^= 1;
-              }
-              tc_fence_after();
-              // (a descriptor's low bits are the address / 16)
-              const uint64_t dq = smem_desc(base + i * Sh::kRows, 16, 1024), dk = smem_desc(at(k), 16, 1024);
-#pragma unroll
-              for (int x = 0; x < DP / 16; ++x) {
-                constexpr int kStep = Sh::kPanel / 16;
-                mma_f16_ss(tmem + i * kTile, dq + (x / 4 * kStep + x % 4 * 2), dk + (x / 4 * kStep + x % 4 * 2), id_s, x > 0);
-              }
-              mma_commit(s_full + i);
-              if (j == nb - 1) mma_commit(q_empty + i);
-            }
+            __syncwarp();
+            if (!Sh::kBeside && !last) score(i, kt, false, j + 1 == nb0 - 1);
           }
-          if (j > 0) mma_commit(kv_empty + v % Sh::kSlots);
-          if (j < nb) mma_commit(kv_empty + k % Sh::kSlots);
+          free_kv(vt);
+          if (!Sh::kBeside && !last) free_kv(kt);
         }
-        g += 2 * nb;
+        r += 2 * nb0;
+        it += gridDim.x;
+        more = seek();
+        if (more) {
+          for (int i = 0; i < tiles; ++i) score(i, r, true, nb == 1);
+          free_kv(r);
+        }
       }
     }
   } else if (warp == 9) {

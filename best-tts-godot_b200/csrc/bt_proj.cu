@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
       if (c0 < cols) mm_ld<kChunk>(acc + c0, r);
 #pragma unroll 1
       for (int i = 0; c0 < cols; ++i, c0 += 4 * kChunk) {
-        tc_wait_ld();
+        tc_loaded(r);
         float y[kChunk];
         const float4* t4 = reinterpret_cast<const float4*>(ts + i * kChunk);
 #pragma unroll
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
         for (int c0 = ((warp - 2) >> 2) * CH; c0 < cols; c0 += 4 * CH) {
           uint32_t r[CH];
           tmem_ld16(tmem + c0 + ((uint32_t)(quad * 32) << 16), r);
-          tc_wait_ld();
+          tc_loaded(r);
 #pragma unroll
           for (int j = 0; j < CH; ++j) {
             const int c = c0 + j, owner = c % S;
