@@ -594,6 +594,252 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if (warp == 8) tmem_free<1>(tmem, 512);
 }
 
+// ---- few queries ---------------------------------------------------------------
+// A step of generation: the queries that share a key head (Tq of each of its
+// G query heads) are rows of one or a few 16-row tiles, and the time is that
+// of reading K and V once.  A warp takes 16 keys at a time, straight from
+// global memory into the operands of 16 x 8 x 16 products (far below the
+// tensor cores' rate here, and free of shared memory):
+//   S = Q K^T  the order of the summed dims is free, so a lane's 16 bytes of a
+//              key row are dims 8c..8c+7 of two products, Q permuted alike;
+//   O += P V   a lane holds dims 8q..8q+7 of the four keys its weights belong
+//              to, and pairs the keys' values register by register; the
+//              order of the result's columns is free as well.
+// Warps, and the CTAs of a cluster, share the keys out and join their
+// (maximum, sum, O) at the end, in a fixed order: through shared memory, and
+// the cluster's shared memory.  No workspace, one launch.
+constexpr int kFewWarps = 4, kFewRows = 16, kFewMax = 64;
+
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int DP>
+struct FewShape {
+  static constexpr int kO = DP / 8;                           // 8-column tiles of O
+  static constexpr int kPitch = DP + 4;                       // a row of partial O, then its maximum and sum
+  static constexpr int kPart = kFewRows * kPitch;             // floats of one part
+  static constexpr int kSmem = kFewWarps * kPart * 4;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
+  using Sh = FewShape<DP>;
+  extern __shared__ float few_sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
+  const unsigned part = S > 1 ? cluster_rank() : 0;
+  uint32_t u = blockIdx.x / (unsigned)S;
+  const int rt = (int)(u % (unsigned)row_tiles);
+  u /= (unsigned)row_tiles;
+  const int64_t Hk = A.H / A.G, b = u / (uint32_t)Hk, hk = u - b * Hk;
+  const int64_t rows = A.G * A.Tq;
+  const int n = (int)keys_of(A, b);
+  const uint8_t* mask = A.mask ? A.mask + b * A.mask_sb : nullptr;
+  const __half* kp = (const __half*)A.k + b * A.ks[0] + hk * A.ks[1];
+  const __half* vp = (const __half*)A.v + b * A.vs[0] + hk * A.vs[1];
+
+  // Q: rows q and q + 8 of the tile, dims 32 x + 8 c ..
+  uint32_t qa[DP / 16][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t r = (int64_t)rt * kFewRows + q + 8 * h;
+    const __half* qp = (const __half*)A.q + b * A.qs[0] + (hk * A.G + r / A.Tq) * A.qs[1] + r % A.Tq * A.qs[2];
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < rows && 32 * x + 8 * c < A.D) v = *reinterpret_cast<const uint4*>(qp + 32 * x + 8 * c);
+      qa[2 * x][h] = v.x;
+      qa[2 * x][2 + h] = v.y;
+      qa[2 * x + 1][h] = v.z;
+      qa[2 * x + 1][2 + h] = v.w;
+    }
+  }
+  float o[Sh::kO][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  const float cs = A.scale * 1.4426950408889634f;   // log2(e)
+
+  // this CTA's keys: whole steps of 16, as even as they go
+  const int steps = (n + 15) / 16;
+  const int s0 = (int)((int64_t)steps * part / S), s1 = (int)((int64_t)steps * (part + 1) / S);
+  for (int st = s0 + warp; st < s1; st += kFewWarps) {
+    const int k0 = 16 * st;
+    uint4 kr[2][DP / 32], vr[4][DP / 64];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = k0 + 8 * h + q;
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x)
+        kr[h][x] = key < n && 32 * x + 8 * c < A.D ? __ldg(reinterpret_cast<const uint4*>(kp + key * A.ks[2] + 32 * x + 8 * c))
+                                                   : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int key = k0 + 2 * c + (y & 1) + 8 * (y >> 1);
+#pragma unroll
+      for (int x = 0; x < DP / 64; ++x)
+        vr[y][x] = key < n && 64 * x + 8 * q < A.D ? __ldg(reinterpret_cast<const uint4*>(vp + key * A.vs[2] + 64 * x + 8 * q))
+                                                   : make_uint4(0, 0, 0, 0);
+    }
+    bool in[4] = {true, true, true, true};   // keys 2 c, 2 c + 1 of each eight
+    if (mask || k0 + 16 > n) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int key = k0 + 2 * c + (y & 1) + 8 * (y >> 1);
+        in[y] = key < n && (!mask || mask[key * A.mask_sk]);
+      }
+    }
+    float s[2][4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 0; x < DP / 32; ++x) {
+        mma_16x8x16(s[h], qa[2 * x], kr[h][x].x, kr[h][x].y);
+        mma_16x8x16(s[h], qa[2 * x + 1], kr[h][x].z, kr[h][x].w);
+      }
+    // scores of rows q (s[.][0, 1]) and q + 8 (s[.][2, 3]), keys 2 c, 2 c + 1 of each eight
+    if (mask || k0 + 16 > n) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (!in[y]) {
+          s[y >> 1][y & 1] = s[y >> 1][2 + (y & 1)] = -INFINITY;
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x) vr[y][x] = make_uint4(0, 0, 0, 0);   // whatever V holds there
+        }
+    }
+    uint32_t pa[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // row q + 8 h
+      // (a NaN score makes the maximum, and so the row, NaN)
+      float top = max3(max3(s[0][2 * h], s[0][2 * h + 1], s[1][2 * h]), s[1][2 * h + 1], m[h]);
+      top = max3(top, __shfl_xor_sync(0xffffffffu, top, 1), -INFINITY);
+      const float mn = max3(top, __shfl_xor_sync(0xffffffffu, top, 2), -INFINITY);
+      const float base = mn == -INFINITY ? 0.0f : mn * cs;
+      if (__any_sync(0xffffffffu, !(mn <= m[h]))) {
+        const float keep = exp2f(m[h] * cs - base);   // (m = -inf: 0)
+        m[h] = mn;
+        l[h] *= keep;
+#pragma unroll
+        for (int i = 0; i < Sh::kO; ++i) {
+          o[i][2 * h] *= keep;
+          o[i][2 * h + 1] *= keep;
+        }
+      }
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = exp2f(fmaf(s[e >> 1][2 * h + (e & 1)], cs, -base));
+        l[h] += p[e];
+      }
+      // weights as float16, lifted by 2^7 off its subnormals (the sum is of
+      // the unrounded ones, lifted alike where the parts are joined)
+      const __half2 h0 = __floats2half2_rn(p[0] * 128.0f, p[1] * 128.0f), h1 = __floats2half2_rn(p[2] * 128.0f, p[3] * 128.0f);
+      pa[h] = *reinterpret_cast<const uint32_t*>(&h0);
+      pa[2 + h] = *reinterpret_cast<const uint32_t*>(&h1);
+    }
+#pragma unroll
+    for (int x = 0; x < DP / 64; ++x) {
+      const uint32_t* v0 = &vr[0][x].x;
+      const uint32_t* v1 = &vr[1][x].x;
+      const uint32_t* v2 = &vr[2][x].x;
+      const uint32_t* v3 = &vr[3][x].x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // dims 64 x + 8 q + 2 i and + 1
+        mma_16x8x16(o[8 * x + 2 * i], pa, __byte_perm(v0[i], v1[i], 0x5410), __byte_perm(v2[i], v3[i], 0x5410));
+        mma_16x8x16(o[8 * x + 2 * i + 1], pa, __byte_perm(v0[i], v1[i], 0x7632), __byte_perm(v2[i], v3[i], 0x7632));
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+  }
+  // the warp's part: O[row][dim], then the maximum and the sum.  Column 2 c + e
+  // of 8-column tile 8 x + j is dim 64 x + 8 (2 c + e) + j.
+  float* mine = few_sm + warp * Sh::kPart;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float* row = mine + (q + 8 * h) * Sh::kPitch;
+#pragma unroll
+    for (int i = 0; i < Sh::kO; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) row[64 * (i / 8) + 8 * (2 * c + e) + i % 8] = o[i][2 * h + e];
+    if (c == 0) {
+      row[DP] = m[h];
+      row[DP + 1] = l[h];
+    }
+  }
+  __syncthreads();
+  // Every thread joins the parts of a share of the outputs: warps of this
+  // CTA, or, in a cluster, of all its CTAs (each CTA the rows r = part mod S).
+  if (S > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const unsigned sm_addr = smem_u32(few_sm);
+  for (int i = threadIdx.x; i < kFewRows * DP; i += 32 * kFewWarps) {
+    const int r = i / DP, d = i % DP;
+    const int64_t gr = (int64_t)rt * kFewRows + r;
+    if (d >= A.D || gr >= rows || r % S != (int)part) continue;
+    float mx = -INFINITY;
+    auto at = [&](int rank, int w, int col) {
+      const unsigned off = (unsigned)(w * Sh::kPart + r * Sh::kPitch + col) * 4;
+      if (S == 1) return few_sm[w * Sh::kPart + r * Sh::kPitch + col];
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr(sm_addr + off, rank)) : "memory");
+      return v;
+    };
+    for (int k = 0; k < S; ++k)
+      for (int w = 0; w < kFewWarps; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
+    float num = 0.0f, den = 0.0f;
+    if (mx != -INFINITY)
+      for (int k = 0; k < S; ++k)
+        for (int w = 0; w < kFewWarps; ++w) {
+          const float pm = at(k, w, DP);
+          const float f = pm == -INFINITY ? 0.0f : exp2f((pm - mx) * cs);
+          num = fmaf(at(k, w, d), f, num);
+          den = fmaf(at(k, w, DP + 1), f, den);
+        }
+    const float y = mx == -INFINITY ? 0.0f : num / (den * 128.0f);
+    __half* out = (__half*)A.out + b * A.os[0] + (hk * A.G + gr / A.Tq) * A.os[1] + gr % A.Tq * A.os[2];
+    out[d * A.os[3]] = __float2half_rn(y);
+  }
+  if (S > 1) {   // no CTA of the cluster leaves while its shared memory is read
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+// Rows of 16-byte pieces that the loads above can take.
+bool rows16(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, int64_t D) {
+  return ((uintptr_t)p & 15) == 0 && (D == 1 || st[3] == 1) && D % 8 == 0 && (B == 1 || st[0] % 8 == 0) &&
+         (H == 1 || st[1] % 8 == 0) && (T == 1 || st[2] % 8 == 0);
+}
+
+template <int DP>
+int attn_few_launch(const AttnArgs& A, int64_t units, int S, int row_tiles) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * S));
+  cfg.blockDim = dim3(32 * kFewWarps);
+  cfg.dynamicSmemBytes = FewShape<DP>::kSmem;
+  cfg.stream = cur_stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)S, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_few_kernel<DP>, A, S, row_tiles);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(BT_ECUDA, "bt_attention: launch failed: %s", cudaGetErrorString(e));
+  }
+  return BT_OK;
+}
+
 // A tensor map over [B, H, T, D] (innermost D), 64 x 128 boxes; false where
 // the strides or the base do not suit one.  mul: 0 for a broadcast head or
 // batch axis, whose extent in the map is 1.
@@ -699,7 +945,18 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   A.out = out->data;
   DevInfo di;
   if ((rc = dev_info(&di))) return rc;
-  if (q->dtype == BT_F16 && A.Tk > 0 && A.Tq > 16) {
+  // Few rows to a key head: by products of 16 rows straight from global
+  // memory, the keys split over a cluster until the GPU is full or a warp is
+  // down to four steps of 16 keys.
+  if (q->dtype == BT_F16 && A.Tk > 0 && A.G * A.Tq <= kFewMax && rows16(A.q, A.qs, A.B, A.H, A.Tq, D) &&
+      rows16(A.k, A.ks, A.B, Hk, A.Tk, D) && rows16(A.v, A.vs, A.B, Hk, A.Tk, D)) {
+    const int64_t row_tiles = (A.G * A.Tq + kFewRows - 1) / kFewRows, units = A.B * Hk * row_tiles;
+    int S = 1;
+    while (S < 8 && units * S < 4 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * kFewWarps * 64) S *= 2;
+    if (units * S < INT32_MAX)
+      return D <= 64 ? attn_few_launch<64>(A, units, S, (int)row_tiles) : attn_few_launch<128>(A, units, S, (int)row_tiles);
+  }
+  if (q->dtype == BT_F16 && A.Tk > 0) {
     AttnTc P{};
     CUtensorMap mq, mk, mv;
     const int64_t q_tiles = (A.Tq + 2 * kTile - 1) / (2 * kTile), items = A.B * A.H * q_tiles;
