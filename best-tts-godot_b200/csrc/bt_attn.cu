@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // Warps, and the CTAs of a cluster, share the keys out and join their
 // (maximum, sum, O) at the end, in a fixed order: through shared memory, and
 // the cluster's shared memory.  No workspace, one launch.
-constexpr int kFewWarps = 4, kFewRows = 16, kFewMax = 64;
+constexpr int kFewWarps = 4, kFewRows = 16, kFewMax = 64, kFewMax32 = 16;
 
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -617,17 +617,68 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int DP>
+// A part of the result in shared memory: ROWS rows of partial O, each with its
+// maximum and sum behind it; one for each warp.
+template <int DP, int ROWS>
 struct FewShape {
   static constexpr int kO = DP / 8;                           // 8-column tiles of O
-  static constexpr int kPitch = DP + 4;                       // a row of partial O, then its maximum and sum
-  static constexpr int kPart = kFewRows * kPitch;             // floats of one part
+  static constexpr int kPitch = DP + 4;
+  static constexpr int kPart = ROWS * kPitch;                 // floats
   static constexpr int kSmem = kFewWarps * kPart * 4;
 };
 
+// Joins the parts of all warps of the CTA, or of the cluster (each CTA then
+// takes the rows r = rank mod S), and stores the outputs.  The parts' O are
+// lifted by `lift` against their sums.
+template <int DP, int ROWS, typename T>
+__device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, int rank, int64_t b, int64_t hk, int64_t row0,
+                                         float cs, float lift) {
+  using Sh = FewShape<DP, ROWS>;
+  __syncthreads();
+  if (S > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const unsigned sm_addr = smem_u32(sm);
+  const int64_t rows = A.G * A.Tq;
+  for (int i = threadIdx.x; i < ROWS * DP; i += 32 * kFewWarps) {
+    const int r = i / DP, d = i % DP;
+    const int64_t gr = row0 + r;
+    if (d >= A.D || gr >= rows || r % S != rank) continue;
+    auto at = [&](int k, int w, int col) {
+      const int off = w * Sh::kPart + r * Sh::kPitch + col;
+      if (S == 1) return sm[off];
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr(sm_addr + off * 4, k)) : "memory");
+      return v;
+    };
+    float mx = -INFINITY;
+    for (int k = 0; k < S; ++k)
+      for (int w = 0; w < kFewWarps; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
+    float num = 0.0f, den = 0.0f;
+    if (mx != -INFINITY)
+      for (int k = 0; k < S; ++k)
+        for (int w = 0; w < kFewWarps; ++w) {
+          const float pm = at(k, w, DP);
+          const float f = pm == -INFINITY ? 0.0f : exp2f((pm - mx) * cs);
+          num = fmaf(at(k, w, d), f, num);
+          den = fmaf(at(k, w, DP + 1), f, den);
+        }
+    const float y = mx == -INFINITY ? 0.0f : num / (den * lift);
+    T* out = (T*)A.out + b * A.os[0] + (hk * A.G + gr / A.Tq) * A.os[1] + gr % A.Tq * A.os[2];
+    if constexpr (sizeof(T) == 2) out[d * A.os[3]] = __float2half_rn(y);
+    else out[d * A.os[3]] = y;
+  }
+  if (S > 1) {   // no CTA of the cluster leaves while its shared memory is read
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
 template <int DP>
 __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
-  using Sh = FewShape<DP>;
+  using Sh = FewShape<DP, kFewRows>;
   extern __shared__ float few_sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
   const unsigned part = S > 1 ? cluster_rank() : 0;
@@ -772,67 +823,324 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
       row[DP + 1] = l[h];
     }
   }
-  __syncthreads();
-  // Every thread joins the parts of a share of the outputs: warps of this
-  // CTA, or, in a cluster, of all its CTAs (each CTA the rows r = part mod S).
-  if (S > 1) {
-    cluster_arrive();
-    cluster_wait();
-  }
-  const unsigned sm_addr = smem_u32(few_sm);
-  for (int i = threadIdx.x; i < kFewRows * DP; i += 32 * kFewWarps) {
-    const int r = i / DP, d = i % DP;
-    const int64_t gr = (int64_t)rt * kFewRows + r;
-    if (d >= A.D || gr >= rows || r % S != (int)part) continue;
-    float mx = -INFINITY;
-    auto at = [&](int rank, int w, int col) {
-      const unsigned off = (unsigned)(w * Sh::kPart + r * Sh::kPitch + col) * 4;
-      if (S == 1) return few_sm[w * Sh::kPart + r * Sh::kPitch + col];
-      float v;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(cluster_addr(sm_addr + off, rank)) : "memory");
-      return v;
-    };
-    for (int k = 0; k < S; ++k)
-      for (int w = 0; w < kFewWarps; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
-    float num = 0.0f, den = 0.0f;
-    if (mx != -INFINITY)
-      for (int k = 0; k < S; ++k)
-        for (int w = 0; w < kFewWarps; ++w) {
-          const float pm = at(k, w, DP);
-          const float f = pm == -INFINITY ? 0.0f : exp2f((pm - mx) * cs);
-          num = fmaf(at(k, w, d), f, num);
-          den = fmaf(at(k, w, DP + 1), f, den);
-        }
-    const float y = mx == -INFINITY ? 0.0f : num / (den * 128.0f);
-    __half* out = (__half*)A.out + b * A.os[0] + (hk * A.G + gr / A.Tq) * A.os[1] + gr % A.Tq * A.os[2];
-    out[d * A.os[3]] = __float2half_rn(y);
-  }
-  if (S > 1) {   // no CTA of the cluster leaves while its shared memory is read
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-  }
+  few_join<DP, kFewRows, __half>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * kFewRows, cs, 128.0f);
 }
 
-// Rows of 16-byte pieces that the loads above can take.
-bool rows16(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, int64_t D) {
-  return ((uintptr_t)p & 15) == 0 && (D == 1 || st[3] == 1) && D % 8 == 0 && (B == 1 || st[0] % 8 == 0) &&
-         (H == 1 || st[1] % 8 == 0) && (T == 1 || st[2] % 8 == 0);
+// The float32 form, for rows of up to 4 queries at a time: eight lanes share a
+// key (a lane holds dims 4 (x + 8 y) .. of Q, K, V and O), four keys a warp
+// step, each of the four lane groups with its own maximum, sum and O.
+constexpr int kFewRows32 = 4;
+
+template <int DP>
+__global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
+  using Sh = FewShape<DP, kFewRows32>;
+  constexpr int R = kFewRows32, Y = DP / 32, kAhead = DP == 64 ? 4 : 2;   // steps of four keys loaded together
+  extern __shared__ float few_sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = lane & 7, grp = lane >> 3;
+  const unsigned part = S > 1 ? cluster_rank() : 0;
+  uint32_t u = blockIdx.x / (unsigned)S;
+  const int rt = (int)(u % (unsigned)row_tiles);
+  u /= (unsigned)row_tiles;
+  const int64_t Hk = A.H / A.G, b = u / (uint32_t)Hk, hk = u - b * Hk;
+  const int64_t rows = A.G * A.Tq;
+  const int n = (int)keys_of(A, b);
+  const uint8_t* mask = A.mask ? A.mask + b * A.mask_sb : nullptr;
+  const float* kp = (const float*)A.k + b * A.ks[0] + hk * A.ks[1];
+  const float* vp = (const float*)A.v + b * A.vs[0] + hk * A.vs[1];
+  const float cs = A.scale * 1.4426950408889634f;   // log2(e)
+  auto ld4 = [&](const float* p, int y, bool in) {
+    const int d = 4 * (x + 8 * y);
+    return in && d < A.D ? __ldg(reinterpret_cast<const float4*>(p + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  };
+  float4 q[R][Y], o[R][Y] = {};
+  float m[R], l[R] = {};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t gr = (int64_t)rt * R + r;
+    m[r] = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < Y; ++y)
+      q[r][y] = ld4((const float*)A.q + b * A.qs[0] + (hk * A.G + gr / A.Tq) * A.qs[1] + gr % A.Tq * A.qs[2], y, gr < rows);
+  }
+  // this CTA's keys: whole steps
+  constexpr int kStep = 4 * kAhead;
+  const int steps = (n + kStep - 1) / kStep;
+  const int s0 = (int)((int64_t)steps * part / S), s1 = (int)((int64_t)steps * (part + 1) / S);
+  for (int st = s0 + warp; st < s1; st += kFewWarps) {
+    float4 k[kAhead][Y], v[kAhead][Y];
+    bool in[kAhead];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      const int key = kStep * st + 4 * t + grp;
+      in[t] = key < n && (!mask || mask[key * A.mask_sk]);
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        k[t][y] = ld4(kp + key * A.ks[2], y, key < n);
+        v[t][y] = ld4(vp + key * A.vs[2], y, key < n);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if ((int64_t)rt * R + r >= rows) break;
+      float s[kAhead], mn = m[r];
+#pragma unroll
+      for (int t = 0; t < kAhead; ++t) {
+        float a = 0.0f;
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          a = fmaf(q[r][y].x, k[t][y].x, a);
+          a = fmaf(q[r][y].y, k[t][y].y, a);
+          a = fmaf(q[r][y].z, k[t][y].z, a);
+          a = fmaf(q[r][y].w, k[t][y].w, a);
+        }
+        a += __shfl_xor_sync(0xffffffffu, a, 1);
+        a += __shfl_xor_sync(0xffffffffu, a, 2);
+        a += __shfl_xor_sync(0xffffffffu, a, 4);
+        s[t] = in[t] ? a : -INFINITY;
+        mn = max3(mn, s[t], -INFINITY);
+      }
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      const float keep = exp2f((m[r] - base) * cs);
+      m[r] = mn;
+      l[r] *= keep;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) o[r][y] = make_float4(o[r][y].x * keep, o[r][y].y * keep, o[r][y].z * keep, o[r][y].w * keep);
+#pragma unroll
+      for (int t = 0; t < kAhead; ++t) {
+        const float p = exp2f((s[t] - base) * cs);
+        l[r] += p;
+        if (!in[t]) continue;   // whatever V holds there
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          o[r][y].x = fmaf(p, v[t][y].x, o[r][y].x);
+          o[r][y].y = fmaf(p, v[t][y].y, o[r][y].y);
+          o[r][y].z = fmaf(p, v[t][y].z, o[r][y].z);
+          o[r][y].w = fmaf(p, v[t][y].w, o[r][y].w);
+        }
+      }
+    }
+  }
+  // the four lane groups of the warp become one part
+  float* mine = few_sm + warp * Sh::kPart;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int z = 8; z <= 16; z *= 2) {
+      const float om = __shfl_xor_sync(0xffffffffu, m[r], z), mn = max3(m[r], om, -INFINITY);
+      const float keep = m[r] == -INFINITY ? 0.0f : exp2f((m[r] - mn) * cs);
+      m[r] = mn;
+      l[r] *= keep;
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], z);
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        float* e = &o[r][y].x;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          e[w] *= keep;
+          e[w] += __shfl_xor_sync(0xffffffffu, e[w], z);
+        }
+      }
+    }
+    if (grp == 0) {
+#pragma unroll
+      for (int y = 0; y < Y; ++y) *reinterpret_cast<float4*>(mine + r * Sh::kPitch + 4 * (x + 8 * y)) = o[r][y];
+      if (x == 0) {
+        mine[r * Sh::kPitch + DP] = m[r];
+        mine[r * Sh::kPitch + DP + 1] = l[r];
+      }
+    }
+  }
+  few_join<DP, R, float>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * R, cs, 1.0f);
+}
+
+// ---- float32 --------------------------------------------------------------------
+// A CTA holds 128 query rows of a head and walks the keys 64 at a time, all
+// arithmetic float32 on the FMA pipe.  Thread (rg, kg) of 16 x 16 owns rows
+// rg + 16 i: of S the keys kg + 16 j, of O the dims kg + 16 j, so a row's
+// maximum is a reduction over sixteen lanes and its rescaling stays with its
+// owner.  Both products run along pairs of the summed axis, two lanes of an
+// fma.f32x2 and added at the end, so no operand has to be doubled: Q and K
+// lie in shared memory as rows of dims, P as rows of keys, V turned round as
+// rows of keys for each dim.  P is exchanged inside the half-warp that owns
+// its rows.  K and V tiles arrive by 4-byte cp.async (any strides; V is turned
+// round on the way; rows of keys that take no part are filled with zeros),
+// the next tile while this one is worked on.  Bound by the FMA pipe.
+constexpr int kRows32 = 128, kKeys32 = 64, kThreads32 = 256;
+
+template <int DP>
+struct Shape32 {
+  static constexpr int kD = DP + 4, kK = kKeys32 + 4;   // pitches: 16-byte reads of 8 rows fall into different banks
+  static constexpr int kQ = kRows32 * kD, kKt = kKeys32 * kD, kVt = DP * kK, kPt = kRows32 * kK;
+  static constexpr int kBufs = DP == 64 ? 2 : 1;
+  static constexpr int kSmem = (kQ + kPt + kBufs * (kKt + kVt)) * 4;
+};
+
+__device__ __forceinline__ void cp_async4_or_zero(unsigned dst, const float* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
 template <int DP>
-int attn_few_launch(const AttnArgs& A, int64_t units, int S, int row_tiles) {
+__global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_constant__ AttnArgs A, int q_tiles) {
+  using Sh = Shape32<DP>;
+  constexpr int J = DP / 16;
+  extern __shared__ __align__(16) float sm32[];
+  float* qs = sm32;
+  float* ps = qs + Sh::kQ;
+  float* kv = ps + Sh::kPt;
+  const int tid = threadIdx.x, lane = tid & 31, kg = lane & 15, rg = tid >> 4;
+  const uint32_t u = blockIdx.x / (unsigned)q_tiles;
+  const int64_t t0 = (int64_t)(blockIdx.x % (unsigned)q_tiles) * kRows32;
+  const int64_t b = u / (uint32_t)A.H, h = u - b * A.H, hk = h / A.G;
+  const int n = (int)keys_of(A, b), D = A.D;
+  const uint8_t* mask = A.mask ? A.mask + b * A.mask_sb : nullptr;
+  const float* qp = (const float*)A.q + b * A.qs[0] + h * A.qs[1] + t0 * A.qs[2];
+  const float* kp = (const float*)A.k + b * A.ks[0] + hk * A.ks[1];
+  const float* vp = (const float*)A.v + b * A.vs[0] + hk * A.vs[1];
+  const int rows = A.Tq - t0 < kRows32 ? (int)(A.Tq - t0) : kRows32;
+  const float cs = A.scale * 1.4426950408889634f;   // log2(e)
+
+  for (int i = tid; i < kRows32 * DP; i += kThreads32) {
+    const int r = i / DP, d = i % DP;
+    const bool in = r < rows && d < D;
+    cp_async4_or_zero(smem_u32(qs + r * Sh::kD + d), in ? qp + r * A.qs[2] + d * A.qs[3] : qp, in);
+  }
+  auto fetch = [&](int k0, int buf) {
+    float* ks = kv + buf * (Sh::kKt + Sh::kVt);
+    float* vs = ks + Sh::kKt;
+    for (int i = tid; i < kKeys32 * DP; i += kThreads32) {
+      const int r = i / DP, d = i % DP, key = k0 + r;
+      const bool in = key < n && d < D, live = in && (!mask || mask[key * A.mask_sk]);
+      cp_async4_or_zero(smem_u32(ks + r * Sh::kD + d), in ? kp + key * A.ks[2] + d * A.ks[3] : kp, in);
+      cp_async4_or_zero(smem_u32(vs + d * Sh::kK + r), live ? vp + key * A.vs[2] + d * A.vs[3] : vp, live);
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+
+  float2 o[8][J] = {};
+  float m[8], l[8] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
+  if (n > 0) fetch(0, 0);
+  for (int k0 = 0, buf = 0; k0 < n; k0 += kKeys32) {
+    const float* ks = kv + buf * (Sh::kKt + Sh::kVt);
+    const float* vs = ks + Sh::kKt;
+    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+    __syncthreads();   // this tile is there, and the last one is read by nobody any more
+    if (Sh::kBufs == 2 && k0 + kKeys32 < n) fetch(k0 + kKeys32, buf ^ 1);
+    bool in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = k0 + kg + 16 * j;
+      in[j] = key < n && (!mask || mask[key * A.mask_sk]);
+    }
+    float2 s2[8][4] = {};
+#pragma unroll(DP == 64 ? 2 : 1)
+    for (int d = 0; d < D; d += 4) {
+      float4 kk[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const float4*>(ks + (kg + 16 * j) * Sh::kD + d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 qq = *reinterpret_cast<const float4*>(qs + (rg + 16 * i) * Sh::kD + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s2[i][j] = pk_fma(make_float2(qq.x, qq.y), make_float2(kk[j].x, kk[j].y), s2[i][j]);
+          s2[i][j] = pk_fma(make_float2(qq.z, qq.w), make_float2(kk[j].z, kk[j].w), s2[i][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s[4], mn = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j] = in[j] ? s2[i][j].x + s2[i][j].y : -INFINITY;
+        mn = max3(mn, s[j], -INFINITY);
+      }
+#pragma unroll
+      for (int z = 1; z < 16; z *= 2) mn = max3(mn, __shfl_xor_sync(0xffffffffu, mn, z), -INFINITY);
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      if (mn != m[i]) {   // (a NaN maximum too)
+        const float keep = exp2f((m[i] - base) * cs);
+        m[i] = mn;
+        l[i] *= keep;
+#pragma unroll
+        for (int j = 0; j < J; ++j) o[i][j] = make_float2(o[i][j].x * keep, o[i][j].y * keep);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p = exp2f((s[j] - base) * cs);
+        l[i] += p;
+        ps[(rg + 16 * i) * Sh::kK + kg + 16 * j] = p;
+      }
+    }
+    __syncwarp();
+#pragma unroll(DP == 64 ? 2 : 1)
+    for (int k = 0; k < kKeys32; k += 4) {
+      float4 vv[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (16 * j < D) vv[j] = *reinterpret_cast<const float4*>(vs + (kg + 16 * j) * Sh::kK + k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 pp = *reinterpret_cast<const float4*>(ps + (rg + 16 * i) * Sh::kK + k);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (16 * j < D) {
+            o[i][j] = pk_fma(make_float2(pp.x, pp.y), make_float2(vv[j].x, vv[j].y), o[i][j]);
+            o[i][j] = pk_fma(make_float2(pp.z, pp.w), make_float2(vv[j].z, vv[j].w), o[i][j]);
+          }
+      }
+    }
+    if (Sh::kBufs == 2) {
+      buf ^= 1;
+    } else {
+      __syncthreads();
+      if (k0 + kKeys32 < n) fetch(k0 + kKeys32, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = rg + 16 * i;
+#pragma unroll
+    for (int z = 1; z < 16; z *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], z);
+    if (r >= rows) continue;
+    float* out = (float*)A.out + b * A.os[0] + h * A.os[1] + (t0 + r) * A.os[2];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (kg + 16 * j < D)
+        out[(kg + 16 * j) * A.os[3]] = m[i] == -INFINITY ? 0.0f : __fdiv_rn(o[i][j].x + o[i][j].y, l[i]);
+  }
+}
+
+template <int DP>
+int attn_f32_launch(const AttnArgs& A, int64_t ctas, int q_tiles) {
+  auto kern = attn_f32_kernel<DP>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape32<DP>::kSmem);
+  if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  kern<<<(unsigned)ctas, kThreads32, Shape32<DP>::kSmem, cur_stream()>>>(A, q_tiles);
+  return check_launch("bt_attention");
+}
+
+// Rows of 16-byte pieces (`per` values each) that the loads above can take.
+bool rows16(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, int64_t D, int per) {
+  return ((uintptr_t)p & 15) == 0 && (D == 1 || st[3] == 1) && D % per == 0 && (B == 1 || st[0] % per == 0) &&
+         (H == 1 || st[1] % per == 0) && (T == 1 || st[2] % per == 0);
+}
+
+template <typename K>
+int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int row_tiles) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * S));
   cfg.blockDim = dim3(32 * kFewWarps);
-  cfg.dynamicSmemBytes = FewShape<DP>::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = cur_stream();
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {(unsigned)S, 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_few_kernel<DP>, A, S, row_tiles);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, A, S, row_tiles);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return set_error(BT_ECUDA, "bt_attention: launch failed: %s", cudaGetErrorString(e));
@@ -945,18 +1253,31 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   A.out = out->data;
   DevInfo di;
   if ((rc = dev_info(&di))) return rc;
-  // Few rows to a key head: by products of 16 rows straight from global
-  // memory, the keys split over a cluster until the GPU is full or a warp is
-  // down to four steps of 16 keys.
-  if (q->dtype == BT_F16 && A.Tk > 0 && A.G * A.Tq <= kFewMax && rows16(A.q, A.qs, A.B, A.H, A.Tq, D) &&
-      rows16(A.k, A.ks, A.B, Hk, A.Tk, D) && rows16(A.v, A.vs, A.B, Hk, A.Tk, D)) {
-    const int64_t row_tiles = (A.G * A.Tq + kFewRows - 1) / kFewRows, units = A.B * Hk * row_tiles;
+  // Few rows to a key head: straight from global memory, the keys split over
+  // a cluster until the GPU is full or a warp is down to four steps of 16.
+  const bool half = q->dtype == BT_F16;
+  const int per = half ? 8 : 4;
+  const int64_t group = A.G * A.Tq;
+  if (A.Tk > 0 && group <= (half ? kFewMax : kFewMax32) && rows16(A.q, A.qs, A.B, A.H, A.Tq, D, per) &&
+      rows16(A.k, A.ks, A.B, Hk, A.Tk, D, per) && rows16(A.v, A.vs, A.B, Hk, A.Tk, D, per)) {
+    const int tile = half ? kFewRows : kFewRows32;
+    const int64_t row_tiles = (group + tile - 1) / tile, units = A.B * Hk * row_tiles;
     int S = 1;
     while (S < 8 && units * S < 4 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * kFewWarps * 64) S *= 2;
-    if (units * S < INT32_MAX)
-      return D <= 64 ? attn_few_launch<64>(A, units, S, (int)row_tiles) : attn_few_launch<128>(A, units, S, (int)row_tiles);
+    if (units * S < INT32_MAX) {
+      if (half)
+        return D <= 64 ? few_launch(attn_few_kernel<64>, FewShape<64, kFewRows>::kSmem, A, units, S, (int)row_tiles)
+                       : few_launch(attn_few_kernel<128>, FewShape<128, kFewRows>::kSmem, A, units, S, (int)row_tiles);
+      return D <= 64 ? few_launch(attn_few32_kernel<64>, FewShape<64, kFewRows32>::kSmem, A, units, S, (int)row_tiles)
+                     : few_launch(attn_few32_kernel<128>, FewShape<128, kFewRows32>::kSmem, A, units, S, (int)row_tiles);
+    }
   }
-  if (q->dtype == BT_F16 && A.Tk > 0) {
+  if (!half && A.Tk > 0) {
+    const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = A.B * A.H * q_tiles;
+    if (ctas < INT32_MAX)
+      return D <= 64 ? attn_f32_launch<64>(A, ctas, (int)q_tiles) : attn_f32_launch<128>(A, ctas, (int)q_tiles);
+  }
+  if (half && A.Tk > 0) {
     AttnTc P{};
     CUtensorMap mq, mk, mv;
     const int64_t q_tiles = (A.Tq + 2 * kTile - 1) / (2 * kTile), items = A.B * A.H * q_tiles;
