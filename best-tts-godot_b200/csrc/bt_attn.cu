@@ -956,33 +956,36 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid
 // ---- float32 --------------------------------------------------------------------
 // A CTA holds 128 query rows of a head and walks the keys 64 at a time, all
 // arithmetic float32 on the FMA pipe.  Thread (rg, kg) of 16 x 16 owns rows
-// rg + 16 i: of S the keys kg + 16 j, of O the dims kg + 16 j, so a row's
-// maximum is a reduction over sixteen lanes and its rescaling stays with its
-// owner.  Both products run along pairs of the summed axis, two lanes of an
-// fma.f32x2 and added at the end, so no operand has to be doubled: Q and K
-// lie in shared memory as rows of dims, P as rows of keys, V turned round as
-// rows of keys for each dim.  P is exchanged inside the half-warp that owns
-// its rows.  K and V tiles arrive by 4-byte cp.async (any strides; V is turned
-// round on the way; rows of keys that take no part are filled with zeros),
+// rg + 16 i: of S the keys kg + 16 j, of O the dims 4 kg .. + 3 (+ 64), so a
+// row's maximum is a reduction over sixteen lanes and its rescaling stays with
+// its owner.  Products run two lanes at a time (fma.f32x2): S along pairs of
+// the summed dims, added at the end; O along pairs of dims, with each weight
+// stored twice.  So Q, K and V lie in shared memory as they come, rows of
+// dims, 16 bytes a read.  P is exchanged inside the half-warp that owns its
+// rows.  K and V tiles arrive by cp.async (16 bytes, or 4 for any strides;
+// rows of keys that take no part are filled with zeros), for dims up to 64
 // the next tile while this one is worked on.  Bound by the FMA pipe.
 constexpr int kRows32 = 128, kKeys32 = 64, kThreads32 = 256;
 
 template <int DP>
 struct Shape32 {
-  static constexpr int kD = DP + 4, kK = kKeys32 + 4;   // pitches: 16-byte reads of 8 rows fall into different banks
-  static constexpr int kQ = kRows32 * kD, kKt = kKeys32 * kD, kVt = DP * kK, kPt = kRows32 * kK;
+  static constexpr int kD = DP + 4;                     // pitch: 16-byte reads of 8 rows fall into different banks
+  static constexpr int kP = 2 * kKeys32 + 4;            // a row of weights, each twice
+  static constexpr int kQ = kRows32 * kD, kKt = kKeys32 * kD, kPt = kRows32 * kP;
   static constexpr int kBufs = DP == 64 ? 2 : 1;
-  static constexpr int kSmem = (kQ + kPt + kBufs * (kKt + kVt)) * 4;
+  static constexpr int kSmem = (kQ + kPt + kBufs * 2 * kKt) * 4;
 };
 
-__device__ __forceinline__ void cp_async4_or_zero(unsigned dst, const float* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+template <int N>
+__device__ __forceinline__ void cp_async_or_zero(unsigned dst, const float* src, bool in) {
+  if constexpr (N == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
-template <int DP>
+template <int DP, int N>   // N: values a copy (4 where every row is 16-byte pieces)
 __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_constant__ AttnArgs A, int q_tiles) {
   using Sh = Shape32<DP>;
-  constexpr int J = DP / 16;
+  constexpr int J = DP / 64;
   extern __shared__ __align__(16) float sm32[];
   float* qs = sm32;
   float* ps = qs + Sh::kQ;
@@ -999,30 +1002,33 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
   const int rows = A.Tq - t0 < kRows32 ? (int)(A.Tq - t0) : kRows32;
   const float cs = A.scale * 1.4426950408889634f;   // log2(e)
 
-  for (int i = tid; i < kRows32 * DP; i += kThreads32) {
-    const int r = i / DP, d = i % DP;
-    const bool in = r < rows && d < D;
-    cp_async4_or_zero(smem_u32(qs + r * Sh::kD + d), in ? qp + r * A.qs[2] + d * A.qs[3] : qp, in);
+  // a thread copies the same dims of every (kThreads32 / kCols)-th row
+  constexpr int kCols = DP / N, kStep = kThreads32 / kCols;
+  const int d0 = tid % kCols * N, r0 = tid / kCols;
+  const bool dim = d0 < D;
+  for (int r = r0; r < kRows32; r += kStep) {
+    const bool in = r < rows && dim;
+    cp_async_or_zero<N>(smem_u32(qs + r * Sh::kD + d0), in ? qp + r * A.qs[2] + d0 * A.qs[3] : qp, in);
   }
   auto fetch = [&](int k0, int buf) {
-    float* ks = kv + buf * (Sh::kKt + Sh::kVt);
-    float* vs = ks + Sh::kKt;
-    for (int i = tid; i < kKeys32 * DP; i += kThreads32) {
-      const int r = i / DP, d = i % DP, key = k0 + r;
-      const bool in = key < n && d < D, live = in && (!mask || mask[key * A.mask_sk]);
-      cp_async4_or_zero(smem_u32(ks + r * Sh::kD + d), in ? kp + key * A.ks[2] + d * A.ks[3] : kp, in);
-      cp_async4_or_zero(smem_u32(vs + d * Sh::kK + r), live ? vp + key * A.vs[2] + d * A.vs[3] : vp, live);
+    float* ks = kv + buf * 2 * Sh::kKt;
+#pragma unroll 4
+    for (int r = r0; r < kKeys32; r += kStep) {
+      const int key = k0 + r;
+      const bool in = key < n && dim, live = in && (!mask || mask[key * A.mask_sk]);
+      cp_async_or_zero<N>(smem_u32(ks + r * Sh::kD + d0), in ? kp + key * A.ks[2] + d0 * A.ks[3] : kp, in);
+      cp_async_or_zero<N>(smem_u32(ks + Sh::kKt + r * Sh::kD + d0), live ? vp + key * A.vs[2] + d0 * A.vs[3] : vp, live);
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 
-  float2 o[8][J] = {};
+  float2 o[8][2 * J] = {};
   float m[8], l[8] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
   if (n > 0) fetch(0, 0);
   for (int k0 = 0, buf = 0; k0 < n; k0 += kKeys32) {
-    const float* ks = kv + buf * (Sh::kKt + Sh::kVt);
+    const float* ks = kv + buf * 2 * Sh::kKt;
     const float* vs = ks + Sh::kKt;
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncthreads();   // this tile is there, and the last one is read by nobody any more
@@ -1065,31 +1071,34 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
         m[i] = mn;
         l[i] *= keep;
 #pragma unroll
-        for (int j = 0; j < J; ++j) o[i][j] = make_float2(o[i][j].x * keep, o[i][j].y * keep);
+        for (int j = 0; j < 2 * J; ++j) o[i][j] = make_float2(o[i][j].x * keep, o[i][j].y * keep);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float p = exp2f((s[j] - base) * cs);
         l[i] += p;
-        ps[(rg + 16 * i) * Sh::kK + kg + 16 * j] = p;
+        *reinterpret_cast<float2*>(ps + (rg + 16 * i) * Sh::kP + 2 * (kg + 16 * j)) = make_float2(p, p);
       }
     }
     __syncwarp();
-#pragma unroll(DP == 64 ? 2 : 1)
-    for (int k = 0; k < kKeys32; k += 4) {
-      float4 vv[J];
+#pragma unroll 2
+    for (int k = 0; k < kKeys32; k += 2) {
+      float4 v0[J], v1[J];
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-        if (16 * j < D) vv[j] = *reinterpret_cast<const float4*>(vs + (kg + 16 * j) * Sh::kK + k);
+      for (int j = 0; j < J; ++j) {
+        v0[j] = *reinterpret_cast<const float4*>(vs + k * Sh::kD + 4 * kg + 64 * j);
+        v1[j] = *reinterpret_cast<const float4*>(vs + (k + 1) * Sh::kD + 4 * kg + 64 * j);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float4 pp = *reinterpret_cast<const float4*>(ps + (rg + 16 * i) * Sh::kK + k);
+        const float4 pp = *reinterpret_cast<const float4*>(ps + (rg + 16 * i) * Sh::kP + 2 * k);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-          if (16 * j < D) {
-            o[i][j] = pk_fma(make_float2(pp.x, pp.y), make_float2(vv[j].x, vv[j].y), o[i][j]);
-            o[i][j] = pk_fma(make_float2(pp.z, pp.w), make_float2(vv[j].z, vv[j].w), o[i][j]);
-          }
+        for (int j = 0; j < J; ++j) {
+          o[i][2 * j] = pk_fma(make_float2(pp.x, pp.y), make_float2(v0[j].x, v0[j].y), o[i][2 * j]);
+          o[i][2 * j + 1] = pk_fma(make_float2(pp.x, pp.y), make_float2(v0[j].z, v0[j].w), o[i][2 * j + 1]);
+          o[i][2 * j] = pk_fma(make_float2(pp.z, pp.w), make_float2(v1[j].x, v1[j].y), o[i][2 * j]);
+          o[i][2 * j + 1] = pk_fma(make_float2(pp.z, pp.w), make_float2(v1[j].z, v1[j].w), o[i][2 * j + 1]);
+        }
       }
     }
     if (Sh::kBufs == 2) {
@@ -1107,15 +1116,17 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
     if (r >= rows) continue;
     float* out = (float*)A.out + b * A.os[0] + h * A.os[1] + (t0 + r) * A.os[2];
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-      if (kg + 16 * j < D)
-        out[(kg + 16 * j) * A.os[3]] = m[i] == -INFINITY ? 0.0f : __fdiv_rn(o[i][j].x + o[i][j].y, l[i]);
+    for (int j = 0; j < 4 * J; ++j) {
+      const int d = 4 * kg + 64 * (j / 4) + j % 4;
+      const float num = j & 1 ? o[i][j / 2].y : o[i][j / 2].x;
+      if (d < D) out[d * A.os[3]] = m[i] == -INFINITY ? 0.0f : __fdiv_rn(num, l[i]);
+    }
   }
 }
 
-template <int DP>
+template <int DP, int N>
 int attn_f32_launch(const AttnArgs& A, int64_t ctas, int q_tiles) {
-  auto kern = attn_f32_kernel<DP>;
+  auto kern = attn_f32_kernel<DP, N>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape32<DP>::kSmem);
   if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
   kern<<<(unsigned)ctas, kThreads32, Shape32<DP>::kSmem, cur_stream()>>>(A, q_tiles);
@@ -1274,8 +1285,12 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   }
   if (!half && A.Tk > 0) {
     const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = A.B * A.H * q_tiles;
+    const bool pieces = rows16(A.q, A.qs, A.B, A.H, A.Tq, D, 4) && rows16(A.k, A.ks, A.B, Hk, A.Tk, D, 4) &&
+                        rows16(A.v, A.vs, A.B, Hk, A.Tk, D, 4);
+    if (ctas < INT32_MAX && pieces)
+      return D <= 64 ? attn_f32_launch<64, 4>(A, ctas, (int)q_tiles) : attn_f32_launch<128, 4>(A, ctas, (int)q_tiles);
     if (ctas < INT32_MAX)
-      return D <= 64 ? attn_f32_launch<64>(A, ctas, (int)q_tiles) : attn_f32_launch<128>(A, ctas, (int)q_tiles);
+      return D <= 64 ? attn_f32_launch<64, 1>(A, ctas, (int)q_tiles) : attn_f32_launch<128, 1>(A, ctas, (int)q_tiles);
   }
   if (half && A.Tk > 0) {
     AttnTc P{};
