@@ -135,6 +135,12 @@ except AttributeError:
     pass
 
 
+_get_device = torch.cuda.current_device
+try:   # the same without the lazy initialisation (a runtime exists, so CUDA is up)
+    _get_device = torch._C._cuda_getDevice
+except AttributeError:
+    pass
+
 _I64x8 = ctypes.c_int64 * 8
 
 
@@ -168,7 +174,7 @@ class BtRuntime:
         self._ew_plans = {}
         self._node_plans = {}   # node signature -> launch plan (see dispatch)
         self._scalars = {}
-        self._local = threading.local()   # per-thread launch plans (see _thread_plans)
+        self._local = threading.local()   # per-thread launch plans (see _plans)
         self.launches = 0
 
     # ---- device values ---------------------------------------------------------
@@ -767,16 +773,20 @@ class BtRuntime:
         return out
 
     # ---- quantised projections and attention -----------------------------------------
-    def _thread_plans(self):
-        """This thread's launch plans.  A plan's descriptors receive the data
-        pointers of each call, so threads do not share them."""
+    # A call looks its launch plan up by the operands' dtypes, shapes, strides
+    # and devices; checks run when a plan is made.  The descriptors of a plan
+    # receive the data pointers of each call, so every thread has its own.
+    def _plans(self, op):
+        local = self._local
         try:
-            return self._local.plans
+            return getattr(local, op)
         except AttributeError:
-            self._local.plans = plans = {}
+            plans = {}
+            setattr(local, op, plans)
             return plans
 
-    def _keep_plan(self, plans, key, plan):
+    @staticmethod
+    def _keep_plan(plans, key, plan):
         if len(plans) >= 4096:
             plans.clear()
         plans[key] = plan
@@ -790,8 +800,8 @@ class BtRuntime:
                 raise ValueError(f"{what}: {name} is on {t.device}, this runtime on {self.device}")
 
     def _call(self, fn, what, *args):
-        """A library call on this runtime's device and the current stream."""
-        if torch.cuda.current_device() != self._index:
+        """A library call on this runtime's device and its current stream."""
+        if _get_device() != self._index:
             with torch.cuda.device(self.device):
                 return self._call(fn, what, *args)
         self.lib.bt_set_stream(_raw_stream(self._index))   # always BT_OK
@@ -808,31 +818,39 @@ class BtRuntime:
         output channels.  q's rows start on 16-byte boundaries (a view of a
         wider buffer where K is not a multiple of 16), as matmul_int8 reads
         them in place."""
-        self._check_here("quantize_rows", x=x)
-        plans = self._thread_plans()
-        key = ("quantize_rows", x.dtype, x.shape, x.stride())
-        plan = plans.get(key)
+        plans = self._plans("quantize_rows")
+        try:
+            key = (x.dtype, x.shape, x.stride(), x.get_device())
+            plan = plans.get(key)
+        except AttributeError:
+            key = plan = None
         if plan is None:
+            self._check_here("quantize_rows", x=x)
             if x.dtype not in (torch.float32, torch.float16):
                 raise TypeError(f"quantize_rows: x must be float32 or float16, not {x.dtype}")
             if x.dim() < 1 or x.shape[-1] == 0:
                 raise ValueError("quantize_rows: rows without values have no largest value")
             if not _one_row_stride(x):
                 return self.quantize_rows(self._contig(x))
-            K = int(x.shape[-1])
-            lead = tuple(int(s) for s in x.shape[:-1])
-            padded = (K + 15) // 16 * 16
-            rows = math.prod(lead)
-            xd = tensor_desc(x)
-            qd = make_tensor(0, np.int8, (rows, K), (padded, 1))
-            plan = self._keep_plan(plans, key, (xd, qd, make_tensor(0, np.float32, (rows,)), lead, padded, K, rows))
-        xd, qd, sd, lead, padded, K, rows = plan
-        q = torch.empty(lead + (padded,), dtype=torch.int8, device=self.device)
-        scale = torch.empty(lead, dtype=torch.float32, device=self.device)
+            lead, K = tuple(int(s) for s in x.shape[:-1]), int(x.shape[-1])
+            padded, rows = (K + 15) // 16 * 16, math.prod(lead)
+            # q's strides: rows of `padded` bytes, C order
+            strides, acc = [1], padded
+            for d in reversed(lead):
+                strides.append(acc)
+                acc *= d
+            plan = self._keep_plan(plans, key, (
+                tensor_desc(x), make_tensor(0, np.int8, (rows, K), (padded, 1)), make_tensor(0, np.float32, (rows,)),
+                lead, tuple(x.shape), tuple(reversed(strides)), _c_strides(lead), rows))
+        xd, qd, sd, lead, shape, q_strides, s_strides, rows = plan
+        q = torch.empty_strided(shape, q_strides, dtype=torch.int8, device=self.device)
+        scale = torch.empty_strided(lead, s_strides, dtype=torch.float32, device=self.device)
         if rows:
-            xd.data, qd.data, sd.data = x.data_ptr(), q.data_ptr(), scale.data_ptr()
+            xd.data = x.data_ptr()
+            qd.data = q.data_ptr()
+            sd.data = scale.data_ptr()
             self._call(self.lib.bt_quantize_rows, "bt_quantize_rows", xd, qd, sd)
-        return (q if padded == K else q[..., :K]), scale
+        return q, scale
 
     def matmul_int8(self, a, a_scale, w, w_scale, bias=None, out_dtype=torch.float32):
         """The product of 8-bit rows with a scale for each token and output
@@ -842,25 +860,33 @@ class BtRuntime:
         (sum_k a w) * a_scale * w_scale + bias as float32 or float16
         [..., N].  The integer sum is exact.  Operands whose rows do not
         start on 16-byte boundaries are copied to such rows first."""
-        self._check_here("matmul_int8", a=a, a_scale=a_scale, w=w, w_scale=w_scale)
-        if bias is not None:
-            self._check_here("matmul_int8", bias=bias)
-        plans = self._thread_plans()
-        key = ("matmul_int8", a.dtype, a.shape, a.stride(), a_scale.dtype, a_scale.shape, a_scale.stride(), w.dtype,
-               w.shape, w.stride(), w_scale.dtype, w_scale.shape, w_scale.stride(),
-               None if bias is None else (bias.dtype, bias.shape, bias.stride()), out_dtype)
-        plan = plans.get(key)
+        plans = self._plans("matmul_int8")
+        try:
+            key = (a.shape, a.stride(), a.dtype, a.get_device(), a_scale.shape, a_scale.stride(), a_scale.dtype,
+                   a_scale.get_device(), w.shape, w.stride(), w.dtype, w.get_device(), w_scale.shape, w_scale.stride(),
+                   w_scale.dtype, w_scale.get_device(), out_dtype,
+                   bias if bias is None else (bias.shape, bias.stride(), bias.dtype, bias.get_device()))
+            plan = plans.get(key)
+        except AttributeError:
+            key = plan = None
         if plan is None:
+            self._check_here("matmul_int8", a=a, a_scale=a_scale, w=w, w_scale=w_scale)
+            if bias is not None:
+                self._check_here("matmul_int8", bias=bias)
             plan = self._keep_plan(plans, key, self._matmul_int8_plan(a, a_scale, w, w_scale, bias, out_dtype))
-        ad, asd, wd, wsd, bd, od, shape, fits = plan
-        if not fits or (a.data_ptr() | w.data_ptr()) & 15:
+        ad, asd, wd, wsd, bd, od, shape, strides, fits, numel = plan
+        pa, pw = a.data_ptr(), w.data_ptr()
+        if not fits or (pa | pw) & 15:
             a2, w2 = self._aligned_rows(a), self._aligned_rows(w)
             s2 = a_scale if a_scale.is_contiguous() else self._contig(a_scale)
             if a2 is not a or w2 is not w or s2 is not a_scale:
                 return self.matmul_int8(a2, s2, w2, w_scale, bias, out_dtype)
-        out = torch.empty(shape, dtype=out_dtype, device=self.device)
-        if out.numel():
-            ad.data, asd.data, wd.data, wsd.data = a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr()
+        out = torch.empty_strided(shape, strides, dtype=out_dtype, device=self.device)
+        if numel:
+            ad.data = pa
+            asd.data = a_scale.data_ptr()
+            wd.data = pw
+            wsd.data = w_scale.data_ptr()
             od.data = out.data_ptr()
             if bias is not None:
                 bd.data = bias.data_ptr()
@@ -891,7 +917,8 @@ class BtRuntime:
         fits = _row_pitch_ok(a) and _row_pitch_ok(w) and a_scale.is_contiguous()
         dt = TORCH_TO_NP[out_dtype]
         return (tensor_desc(a), make_tensor(0, np.float32, (rows,)), tensor_desc(w), tensor_desc(w_scale),
-                None if bias is None else tensor_desc(bias), make_tensor(0, dt, (rows, N)), lead + (N,), fits)
+                None if bias is None else tensor_desc(bias), make_tensor(0, dt, (rows, N)), lead + (N,),
+                _c_strides(lead + (N,)), fits, rows * N)
 
     def _aligned_rows(self, t):
         """t itself where its rows have one stride, a multiple of 16 bytes,
@@ -913,23 +940,30 @@ class BtRuntime:
         gives zeros.  scale defaults to 1 / sqrt(D).  Views of any strides
         are read in place (a [B, T, H, D] projection permuted to
         [B, H, T, D])."""
-        self._check_here("attention", q=q, k=k, v=v)
-        if lengths is not None:
-            self._check_here("attention", lengths=lengths)
-        if key_mask is not None:
-            self._check_here("attention", key_mask=key_mask)
-        plans = self._thread_plans()
-        key = ("attention", q.dtype, q.shape, q.stride(), k.dtype, k.shape, k.stride(), v.dtype, v.shape, v.stride(),
-               None if lengths is None else (lengths.dtype, lengths.shape, lengths.stride()),
-               None if key_mask is None else (key_mask.dtype, key_mask.shape, key_mask.stride()),
-               scale)
-        plan = plans.get(key)
+        plans = self._plans("attention")
+        try:
+            key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape,
+                   v.stride(), v.dtype, v.get_device(), scale,
+                   lengths if lengths is None else (lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device()),
+                   key_mask if key_mask is None else (key_mask.shape, key_mask.stride(), key_mask.dtype,
+                                                      key_mask.get_device()))
+            plan = plans.get(key)
+        except AttributeError:
+            key = plan = None
         if plan is None:
+            self._check_here("attention", q=q, k=k, v=v)
+            if lengths is not None:
+                self._check_here("attention", lengths=lengths)
+            if key_mask is not None:
+                self._check_here("attention", key_mask=key_mask)
             plan = self._keep_plan(plans, key, self._attention_plan(q, k, v, lengths, key_mask, scale))
-        qd, kd, vd, ld, md, od, sc, shape, strides = plan
+        qd, kd, vd, ld, md, od, sc, shape, strides, numel = plan
         out = torch.empty_strided(shape, strides, dtype=q.dtype, device=self.device)
-        if out.numel():
-            qd.data, kd.data, vd.data, od.data = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        if numel:
+            qd.data = q.data_ptr()
+            kd.data = k.data_ptr()
+            vd.data = v.data_ptr()
+            od.data = out.data_ptr()
             if lengths is not None:
                 ld.data = lengths.data_ptr()
             if key_mask is not None:
@@ -966,7 +1000,7 @@ class BtRuntime:
             acc *= shape[ax]
         od = make_tensor(0, np_dtype(q), shape, strides)
         return (tensor_desc(q), tensor_desc(k), tensor_desc(v), None if lengths is None else tensor_desc(lengths),
-                None if key_mask is None else tensor_desc(key_mask), od, scale, shape, tuple(strides))
+                None if key_mask is None else tensor_desc(key_mask), od, scale, shape, tuple(strides), math.prod(shape))
 
     def _as_f32(self, t):
         dt = np_dtype(t)
@@ -1395,6 +1429,14 @@ def _one_row_stride(t):
                 return False
             n *= int(t.shape[d])
     return True
+
+
+def _c_strides(shape):
+    strides, acc = [], 1
+    for d in reversed(shape):
+        strides.append(acc)
+        acc *= d
+    return tuple(reversed(strides))
 
 
 def _row_pitch_ok(t):

@@ -50,6 +50,14 @@ __device__ __forceinline__ float ldf(const T* p) {
   else return *p;
 }
 
+// 2^x by the special-function unit (relative error 2^-22.5; results below
+// 2^-126 become 0).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // One warp per query row, any strides: a lane scores one key of 32, then the
 // lanes share the output's dimensions.
 constexpr int kRowWarps = 4;
@@ -769,7 +777,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
       const float mn = max3(top, __shfl_xor_sync(0xffffffffu, top, 2), -INFINITY);
       const float base = mn == -INFINITY ? 0.0f : mn * cs;
       if (__any_sync(0xffffffffu, !(mn <= m[h]))) {
-        const float keep = exp2f(m[h] * cs - base);   // (m = -inf: 0)
+        const float keep = ex2(m[h] * cs - base);   // (m = -inf: 0)
         m[h] = mn;
         l[h] *= keep;
 #pragma unroll
@@ -781,7 +789,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[e] = exp2f(fmaf(s[e >> 1][2 * h + (e & 1)], cs, -base));
+        p[e] = ex2(fmaf(s[e >> 1][2 * h + (e & 1)], cs, -base));
         l[h] += p[e];
       }
       // weights as float16, lifted by 2^7 off its subnormals (the sum is of
@@ -900,14 +908,14 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid
         mn = max3(mn, s[t], -INFINITY);
       }
       const float base = mn == -INFINITY ? 0.0f : mn;
-      const float keep = exp2f((m[r] - base) * cs);
+      const float keep = ex2((m[r] - base) * cs);
       m[r] = mn;
       l[r] *= keep;
 #pragma unroll
       for (int y = 0; y < Y; ++y) o[r][y] = make_float4(o[r][y].x * keep, o[r][y].y * keep, o[r][y].z * keep, o[r][y].w * keep);
 #pragma unroll
       for (int t = 0; t < kAhead; ++t) {
-        const float p = exp2f((s[t] - base) * cs);
+        const float p = ex2((s[t] - base) * cs);
         l[r] += p;
         if (!in[t]) continue;   // whatever V holds there
 #pragma unroll
@@ -1067,7 +1075,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       for (int z = 1; z < 16; z *= 2) mn = max3(mn, __shfl_xor_sync(0xffffffffu, mn, z), -INFINITY);
       const float base = mn == -INFINITY ? 0.0f : mn;
       if (mn != m[i]) {   // (a NaN maximum too)
-        const float keep = exp2f((m[i] - base) * cs);
+        const float keep = ex2((m[i] - base) * cs);
         m[i] = mn;
         l[i] *= keep;
 #pragma unroll
@@ -1075,7 +1083,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = exp2f((s[j] - base) * cs);
+        const float p = ex2((s[j] - base) * cs);
         l[i] += p;
         *reinterpret_cast<float2*>(ps + (rg + 16 * i) * Sh::kP + 2 * (kg + 16 * j)) = make_float2(p, p);
       }
