@@ -126,9 +126,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // float16 weights P (D <= 64: beside S; else over S) and the 128 x D output O.
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a query row, reads its
 //                   128 scores into registers, writes its weights
-//   warp 8          issues S = Q K^T and O += P V (P read from tensor memory)
-//   warp 9          TMA loads: the item's Q tiles, a ring of K and V tiles
-//   warp 10         zeroes the rows of V whose keys take no part (only where
+//   warps 8, 9      issue tile 0's, 1's S = Q K^T and O += P V (P read from
+//                   tensor memory); one warp for both was the bottleneck: its
+//                   waits and commits alone took 2000 clocks a key tile
+//   warp 10         TMA loads: the item's Q tiles, a ring of K and V tiles
+//   warp 11         zeroes the rows of V whose keys take no part (only where
 //                   there are lengths or a mask: a weight of 0 times NaN
 //                   would not be 0)
 // The two tiles take turns: while one's softmax runs, the tensor cores work
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 constexpr int kTile = 128;
 constexpr int kAttnThreads = 384;
 constexpr float kGrow = 8.0f, kLift = 7.0f;
-constexpr int kPolyOf8 = 2;   // of eight pairs of weights, those on the FMA pipe
+constexpr int kPolyOf8 = 0;   // of eight pairs of weights, those on the FMA pipe
 
 struct AttnTc {
   AttnArgs a;
@@ -209,6 +211,22 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
+// The same operations where they are written: the order is the schedule.
+__device__ __forceinline__ float2 pk_fma_v(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm volatile("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+               "mov.b64 rc, {%6, %7};\n\tfma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+               : "=f"(d.x), "=f"(d.y)
+               : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ void ex2_v(float& x) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x)); }
+__device__ __forceinline__ uint32_t cvt_v(float2 x) {
+  uint32_t h;
+  asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(x.y), "f"(x.x));
+  return h;
+}
+
 struct ItemPos {
   int64_t b;
   int h, t0;
@@ -220,6 +238,12 @@ __device__ __forceinline__ ItemPos item_pos(const AttnTc& A, uint32_t it) {
   p.b = head / (uint32_t)A.a.H;
   p.h = (int)(head - (uint32_t)p.b * (uint32_t)A.a.H);
   return p;
+}
+
+// The keys of an item's batch entry (0 past the last item), asked for an item
+// ahead by every role: the load's latency would stand before each item.
+__device__ __forceinline__ int item_keys(const AttnTc& A, uint32_t it) {
+  return it < A.items ? (int)keys_of(A.a, item_pos(A, it).b) : 0;
 }
 
 template <int DP>
@@ -254,7 +278,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
       mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
+      mbar_init(kv_empty + i, 2);
       mbar_init(v_ok + i, 1);
     }
     tma_prefetch(&map_q);
@@ -270,16 +294,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if (warp < 8) {
     const int tile = warp >> 2;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n");   // 256 x 208 + 128 x 88 = 384 x 168
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");   // 256 x 216 + 128 x 72 = 384 x 168
     const uint32_t sp = tmem + tile * kTile + lanes, pp = tmem + Sh::kP + tile * Sh::kPStep + lanes;
     const uint32_t op = tmem + Sh::kO + tile * DP + lanes;
     const float c = a.scale * 1.4426950408889634f;   // log2(e)
+    // Tile 0 and 1 take turns at the exponentials (see above): a warpgroup
+    // waits for its turn and then passes it on, tile 0 first.
+    auto my_turn = [&]() { asm volatile("bar.sync %0, 256;\n" ::"r"(1 + tile) : "memory"); };
+    auto your_turn = [&]() { asm volatile("bar.arrive %0, 256;\n" ::"r"(2 - tile) : "memory"); };
+    if (tile == 1) your_turn();
     uint32_t g = 0;   // key tiles this query tile has worked on
+    int n_next = item_keys(A, blockIdx.x);
     for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
       const ItemPos pos = item_pos(A, it);
+      const int n = n_next;
+      n_next = item_keys(A, it + gridDim.x);
       const int64_t t = pos.t0 + tile * kTile + (warp & 3) * 32 + lane;
       if (pos.t0 + tile * kTile >= a.Tq) continue;
-      const int n = (int)keys_of(a, pos.b);
+      const bool turns = pos.t0 + kTile < a.Tq;   // both tiles have work
       const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
       float m = -INFINITY, mc = 0.0f;   // the reference (-inf: no key yet) and m c - 7
       float2 l = {0.0f, 0.0f};
@@ -329,6 +361,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         // a NaN among the scores, or +inf (inf - inf), makes the row NaN by
         // way of its reference; the comparisons below are true for NaN
         const bool grow = !(top <= m) && (m == -INFINITY || !((top - m) * c <= kGrow));
+        // (asked for here, needed below)
+        const bool p_free = !Sh::kBeside || k0 == 0 || mbar_try(smem_u32(pv_done + 2 * tile + ((g - 1) & 1)), (g - 1) >> 1 & 1);
         if (__any_sync(0xffffffffu, grow)) {
           if (top == INFINITY) top = NAN;
           // where there was no key before, O and l are 0 or not yet written
@@ -354,29 +388,36 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
           }
         }
+        if (turns) my_turn();
         const float2 c2 = {c, c}, mc2 = {-mc, -mc};
-        float2 part_l[4] = {};
+        float2 part_l[2] = {};
+        // Pair x is scaled in step x, exponentiated in step x + 1, summed and
+        // rounded in step x + 3, in this order (volatile): the special-function
+        // unit takes eight clocks an instruction, and what is issued between
+        // two of its instructions is free.
+        float2 e[64];
+        uint32_t p[4][16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t p[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float2 e = pk_fma(make_float2(__uint_as_float(s[i][2 * j]), __uint_as_float(s[i][2 * j + 1])), c2, mc2);
-            if (j % 8 >= 8 - kPolyOf8) {
-              e = exp2_poly(e);
-            } else {
-              asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
-              asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+        for (int x = 0; x < 64 + 3; ++x) {
+          if (x < 64)
+            e[x] = pk_fma_v(make_float2(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, mc2);
+          const bool poly = x >= 1 && x <= 64 && (x - 1) % 8 >= 8 - kPolyOf8;
+          if (x >= 1 && x <= 64 && !poly) ex2_v(e[x - 1].x);
+          if (x >= 3) part_l[x & 1] = pk_add(part_l[x & 1], e[x - 3]);
+          if (x >= 1 && x <= 64 && !poly) ex2_v(e[x - 1].y);
+          if (poly) e[x - 1] = exp2_poly(e[x - 1]);
+          if (x >= 3) {
+            const int y = x - 3;
+            p[y / 16][y % 16] = cvt_v(e[y]);
+            if (y % 16 == 15) {
+              // (P beside S: the last product has read its weights by now)
+              if (y == 15 && !p_free) tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);
+              tmem_st16(pp + y / 16 * 16, p[y / 16]);   // column j: keys 2 j and 2 j + 1
             }
-            part_l[j & 3] = pk_add(part_l[j & 3], e);
-            const __half2 h = __float22half2_rn(e);
-            p[j] = *reinterpret_cast<const uint32_t*>(&h);
           }
-          // (P beside S: the last product has read its weights by now)
-          if (Sh::kBeside && i == 0 && k0 > 0) tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);
-          tmem_st16(pp + 16 * i, p);   // column j: keys 2 j and 2 j + 1
         }
-        l = pk_add(l, pk_add(pk_add(part_l[0], part_l[1]), pk_add(part_l[2], part_l[3])));
+        if (turns) your_turn();
+        l = pk_add(l, pk_add(part_l[0], part_l[1]));
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -428,105 +469,83 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       tc_fence_before();   // (O is read before this warp's next arrival lets it be written)
     }
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
   }
-  if (warp == 8) {
+  if (warp == 8 || warp == 9) {
     // The whole warp walks the loop and one elected lane issues: the operands
-    // are then known to be uniform (with the loop on one lane, issuing the
-    // sixteen products of a step took 3300 clocks).
-    {
-      constexpr uint32_t id_s = 1u << 4 | (kTile / 8u) << 17 | (kTile / 16u) << 24;
-      constexpr uint32_t id_o = 1u << 4 | 1u << 16 | (DP / 8u) << 17 | (kTile / 16u) << 24;   // V: rows along the sum
-      unsigned q_ph[2] = {0, 0};
-      uint32_t g[2] = {0, 0};   // key tiles scored so far, for each query tile
-      uint32_t r = 0;           // K and V tiles used so far: K tile j of an item is r + 2 j, its V the one after
-      // an item's key and query tiles; the next item with keys from `it` on
-      uint32_t it = blockIdx.x;
-      int nb = 0, tiles = 0;
-      auto seek = [&]() {
-        for (; it < A.items; it += gridDim.x) {
-          const ItemPos pos = item_pos(A, it);
-          nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
-          tiles = pos.t0 + kTile < a.Tq ? 2 : 1;
-          if (nb > 0) return true;
+    // are then known to be uniform (with the loop on one lane, issuing sixteen
+    // products took 3300 clocks).
+    constexpr uint32_t id_s = 1u << 4 | (kTile / 8u) << 17 | (kTile / 16u) << 24;
+    constexpr uint32_t id_o = 1u << 4 | 1u << 16 | (DP / 8u) << 17 | (kTile / 16u) << 24;   // V: rows along the sum
+    const int i = warp - 8;
+    const uint32_t ts = tmem + i * kTile, tp = tmem + Sh::kP + i * Sh::kPStep, to = tmem + Sh::kO + i * DP;
+    const uint64_t dq = smem_desc(base + i * Sh::kRows, 16, 1024);   // (the low bits are the address / 16)
+    unsigned q_ph = 0;
+    uint32_t g = 0, r = 0;   // key tiles scored; K and V tiles used so far: K tile j of an item is r + 2 j, its V the one after
+    auto score = [&](uint32_t kt, bool first, bool last) {
+      const uint32_t slot_k = kt % Sh::kSlots;
+      if (first) {
+        tc_wait(q_full + i, q_ph, aborted);
+        q_ph ^= 1;
+      }
+      tc_wait(kv_full + slot_k, kt / Sh::kSlots & 1, aborted);
+      if (Sh::kBeside && g > 0) tc_wait(s_free + i, (g - 1) & 1, aborted);
+      tc_fence_after();
+      const uint64_t dk = smem_desc(ring + slot_k * Sh::kRows, 16, 1024);
+      if (elect_one()) {
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          constexpr int kStep = Sh::kPanel / 16;
+          mma_f16_ss(ts, dq + (x / 4 * kStep + x % 4 * 2), dk + (x / 4 * kStep + x % 4 * 2), id_s, x > 0);
         }
-        return false;
-      };
-      // S of query tile i and K tile kt
-      auto score = [&](int i, uint32_t kt, bool first, bool last) {
-        if (first) {
-          tc_wait(q_full + i, q_ph[i], aborted);
-          q_ph[i] ^= 1;
+        mma_commit(s_full + i);
+        mma_commit(kv_empty + slot_k);
+        if (last) mma_commit(q_empty + i);
+      }
+      __syncwarp();
+      ++g;
+    };
+    int n_next = item_keys(A, blockIdx.x);
+    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
+      const ItemPos pos = item_pos(A, it);
+      const int nb = (n_next + kTile - 1) / kTile;
+      n_next = item_keys(A, it + gridDim.x);
+      if (pos.t0 + i * kTile >= a.Tq) {   // no such tile in this item: pass its keys on
+        for (int j = 0; j < 2 * nb; ++j, ++r) {
+          tc_wait(kv_full + r % Sh::kSlots, r / Sh::kSlots & 1, aborted);
+          if (lane == 0) mbar_arrive(kv_empty + r % Sh::kSlots);
+          __syncwarp();
         }
-        tc_wait(kv_full + kt % Sh::kSlots, kt / Sh::kSlots & 1, aborted);
-        if (Sh::kBeside && g[i] > 0) tc_wait(s_free + i, (g[i] - 1) & 1, aborted);
+        continue;
+      }
+      if (nb > 0) score(r, true, nb == 1);
+      for (int j = 0; j < nb; ++j, r += 2) {
+        const bool last = j == nb - 1;
+        const uint32_t slot_v = (r + 1) % Sh::kSlots, b = g - 1;
+        if (Sh::kBeside && !last) score(r + 2, false, j + 1 == nb - 1);
+        tc_wait((fix_v ? v_ok : kv_full) + slot_v, (r + 1) / Sh::kSlots & 1, aborted);
+        tc_wait(p_full + i, b & 1, aborted);
         tc_fence_after();
-        // (a descriptor's low bits are the address / 16)
-        const uint64_t dq = smem_desc(base + i * Sh::kRows, 16, 1024), dk = smem_desc(ring + kt % Sh::kSlots * Sh::kRows, 16, 1024);
+        const uint64_t dv = smem_desc(ring + slot_v * Sh::kRows, Sh::kPanel, 1024);
         if (elect_one()) {
 #pragma unroll
-          for (int x = 0; x < DP / 16; ++x) {
-            constexpr int kStep = Sh::kPanel / 16;
-            mma_f16_ss(tmem + i * kTile, dq + (x / 4 * kStep + x % 4 * 2), dk + (x / 4 * kStep + x % 4 * 2), id_s, x > 0);
-          }
-          mma_commit(s_full + i);
-          if (last) mma_commit(q_empty + i);
+          for (int x = 0; x < kTile / 16; ++x) mma_f16_ts(to, tp + 8 * x, dv + 128 * x, id_o, j > 0 || x > 0);
+          mma_commit(pv_done + 2 * i + (b & 1));
+          mma_commit(kv_empty + slot_v);
         }
         __syncwarp();
-        ++g[i];
-      };
-      auto free_kv = [&](uint32_t x) {
-        if (elect_one()) mma_commit(kv_empty + x % Sh::kSlots);
-        __syncwarp();
-      };
-      bool more = seek();
-      if (more) {
-        for (int i = 0; i < tiles; ++i) score(i, r, true, nb == 1);
-        free_kv(r);
-      }
-      while (more) {
-        const int nb0 = nb, tiles0 = tiles;
-        for (int j = 0; j < nb0; ++j) {
-          const bool last = j == nb0 - 1;
-          const uint32_t vt = r + 2 * j + 1, kt = vt + 1;
-          if (Sh::kBeside && !last) {
-            for (int i = 0; i < tiles0; ++i) score(i, kt, false, j + 1 == nb0 - 1);
-            free_kv(kt);
-          }
-          tc_wait((fix_v ? v_ok : kv_full) + vt % Sh::kSlots, vt / Sh::kSlots & 1, aborted);
-          for (int i = 0; i < tiles0; ++i) {
-            const uint32_t b = Sh::kBeside && !last ? g[i] - 2 : g[i] - 1;
-            tc_wait(p_full + i, b & 1, aborted);
-            tc_fence_after();
-            const uint64_t dv = smem_desc(ring + vt % Sh::kSlots * Sh::kRows, Sh::kPanel, 1024);
-            if (elect_one()) {
-#pragma unroll
-              for (int x = 0; x < kTile / 16; ++x)
-                mma_f16_ts(tmem + Sh::kO + i * DP, tmem + Sh::kP + i * Sh::kPStep + 8 * x, dv + 128 * x, id_o, j > 0 || x > 0);
-              mma_commit(pv_done + 2 * i + (b & 1));
-            }
-            __syncwarp();
-            if (!Sh::kBeside && !last) score(i, kt, false, j + 1 == nb0 - 1);
-          }
-          free_kv(vt);
-          if (!Sh::kBeside && !last) free_kv(kt);
-        }
-        r += 2 * nb0;
-        it += gridDim.x;
-        more = seek();
-        if (more) {
-          for (int i = 0; i < tiles; ++i) score(i, r, true, nb == 1);
-          free_kv(r);
-        }
+        if (!Sh::kBeside && !last) score(r + 2, false, j + 1 == nb - 1);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 10) {
     if (lane == 0) {
       unsigned q_ph[2] = {1, 1};
       uint32_t g = 0;
+      int n_next = item_keys(A, blockIdx.x);
       for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
         const ItemPos pos = item_pos(A, it);
-        const int nb = ((int)keys_of(a, pos.b) + kTile - 1) / kTile;
+        const int nb = (n_next + kTile - 1) / kTile;
+        n_next = item_keys(A, it + gridDim.x);
         if (nb == 0) continue;
         const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1, b = (int)pos.b, hk = pos.h / (int)a.G;
         auto load = [&](const CUtensorMap* m, unsigned dst, uint64_t* bar, int t0, int h, int bb) {
@@ -552,11 +571,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_wait(kv_empty + g % Sh::kSlots, (g / Sh::kSlots & 1) ^ 1, aborted);
       for (int i = 0; i < 2; ++i) tc_wait(q_empty + i, q_ph[i], aborted);
     }
-  } else if (warp == 10 && fix_v) {
+  } else if (warp == 11 && fix_v) {
     uint32_t g = 1;
+    int n_next = item_keys(A, blockIdx.x);
     for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
       const ItemPos pos = item_pos(A, it);
-      const int n = (int)keys_of(a, pos.b);
+      const int n = n_next;
+      n_next = item_keys(A, it + gridDim.x);
       const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
       for (int k0 = 0; k0 < n; k0 += kTile, g += 2) {
         bool in[4];
