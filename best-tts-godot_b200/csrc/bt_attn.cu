@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // Warps, and the CTAs of a cluster, share the keys out and join their
 // (maximum, sum, O) at the end, in a fixed order: through shared memory, and
 // the cluster's shared memory.  No workspace, one launch.
-constexpr int kFewWarps = 4, kFewRows = 16, kFewMax = 64, kFewMax32 = 16;
+constexpr int kFewRows = 16, kFewRows32 = 4;
 
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -648,21 +648,21 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
 
 // A part of the result in shared memory: ROWS rows of partial O, each with its
 // maximum and sum behind it; one for each warp.
-template <int DP, int ROWS>
+template <int DP, int ROWS, int W>
 struct FewShape {
   static constexpr int kO = DP / 8;                           // 8-column tiles of O
   static constexpr int kPitch = DP + 4;
   static constexpr int kPart = ROWS * kPitch;                 // floats
-  static constexpr int kSmem = kFewWarps * kPart * 4;
+  static constexpr int kSmem = W * kPart * 4;
 };
 
 // Joins the parts of all warps of the CTA, or of the cluster (each CTA then
 // takes the rows r = rank mod S), and stores the outputs.  The parts' O are
 // lifted by `lift` against their sums.
-template <int DP, int ROWS, typename T>
+template <int DP, int ROWS, int W, typename T>
 __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, int rank, int64_t b, int64_t hk, int64_t row0,
                                          float cs, float lift) {
-  using Sh = FewShape<DP, ROWS>;
+  using Sh = FewShape<DP, ROWS, W>;
   __syncthreads();
   if (S > 1) {
     cluster_arrive();
@@ -670,7 +670,7 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
   }
   const unsigned sm_addr = smem_u32(sm);
   const int64_t rows = A.G * A.Tq;
-  for (int i = threadIdx.x; i < ROWS * DP; i += 32 * kFewWarps) {
+  for (int i = threadIdx.x; i < ROWS * DP; i += 32 * W) {
     const int r = i / DP, d = i % DP;
     const int64_t gr = row0 + r;
     if (d >= A.D || gr >= rows || r % S != rank) continue;
@@ -683,11 +683,11 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
     };
     float mx = -INFINITY;
     for (int k = 0; k < S; ++k)
-      for (int w = 0; w < kFewWarps; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
+      for (int w = 0; w < W; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
     float num = 0.0f, den = 0.0f;
     if (mx != -INFINITY)
       for (int k = 0; k < S; ++k)
-        for (int w = 0; w < kFewWarps; ++w) {
+        for (int w = 0; w < W; ++w) {
           const float pm = at(k, w, DP);
           const float f = pm == -INFINITY ? 0.0f : exp2f((pm - mx) * cs);
           num = fmaf(at(k, w, d), f, num);
@@ -705,9 +705,9 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
   }
 }
 
-template <int DP>
-__global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
-  using Sh = FewShape<DP, kFewRows>;
+template <int DP, int W>
+__global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
+  using Sh = FewShape<DP, kFewRows, W>;
   extern __shared__ float few_sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
   const unsigned part = S > 1 ? cluster_rank() : 0;
@@ -744,9 +744,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
   // this CTA's keys: whole steps of 16, as even as they go
   const int steps = (n + 15) / 16;
   const int s0 = (int)((int64_t)steps * part / S), s1 = (int)((int64_t)steps * (part + 1) / S);
-  for (int st = s0 + warp; st < s1; st += kFewWarps) {
-    const int k0 = 16 * st;
-    uint4 kr[2][DP / 32], vr[4][DP / 64];
+  uint4 kr[2][DP / 32], vr[4][DP / 64];
+  auto load_k = [&](int k0) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int key = k0 + 8 * h + q;
@@ -755,6 +754,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
         kr[h][x] = key < n && 32 * x + 8 * c < A.D ? __ldg(reinterpret_cast<const uint4*>(kp + key * A.ks[2] + 32 * x + 8 * c))
                                                    : make_uint4(0, 0, 0, 0);
     }
+  };
+  if (s0 + warp < s1) load_k(16 * (s0 + warp));
+  for (int st = s0 + warp; st < s1; st += W) {
+    const int k0 = 16 * st;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int key = k0 + 2 * c + (y & 1) + 8 * (y >> 1);
@@ -779,6 +782,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
         mma_16x8x16(s[h], qa[2 * x], kr[h][x].x, kr[h][x].y);
         mma_16x8x16(s[h], qa[2 * x + 1], kr[h][x].z, kr[h][x].w);
       }
+    // the next step's keys, while this one's weights are computed
+    if (st + W < s1) load_k(16 * (st + W));
     // scores of rows q (s[.][0, 1]) and q + 8 (s[.][2, 3]), keys 2 c, 2 c + 1 of each eight
     if (mask || k0 + 16 > n) {
 #pragma unroll
@@ -852,17 +857,15 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few_kernel(const __grid_c
       row[DP + 1] = l[h];
     }
   }
-  few_join<DP, kFewRows, __half>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * kFewRows, cs, 128.0f);
+  few_join<DP, kFewRows, W, __half>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * kFewRows, cs, 128.0f);
 }
 
 // The float32 form, for rows of up to 4 queries at a time: eight lanes share a
 // key (a lane holds dims 4 (x + 8 y) .. of Q, K, V and O), four keys a warp
 // step, each of the four lane groups with its own maximum, sum and O.
-constexpr int kFewRows32 = 4;
-
-template <int DP>
-__global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
-  using Sh = FewShape<DP, kFewRows32>;
+template <int DP, int W>
+__global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
+  using Sh = FewShape<DP, kFewRows32, W>;
   constexpr int R = kFewRows32, Y = DP / 32, kAhead = DP == 64 ? 4 : 2;   // steps of four keys loaded together
   extern __shared__ float few_sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = lane & 7, grp = lane >> 3;
@@ -895,7 +898,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid
   constexpr int kStep = 4 * kAhead;
   const int steps = (n + kStep - 1) / kStep;
   const int s0 = (int)((int64_t)steps * part / S), s1 = (int)((int64_t)steps * (part + 1) / S);
-  for (int st = s0 + warp; st < s1; st += kFewWarps) {
+  for (int st = s0 + warp; st < s1; st += W) {
     float4 k[kAhead][Y], v[kAhead][Y];
     bool in[kAhead];
 #pragma unroll
@@ -979,7 +982,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attn_few32_kernel(const __grid
       }
     }
   }
-  few_join<DP, R, float>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * R, cs, 1.0f);
+  few_join<DP, R, W, float>(A, few_sm, S, (int)part, b, hk, (int64_t)rt * R, cs, 1.0f);
 }
 
 // ---- float32 --------------------------------------------------------------------
@@ -1168,11 +1171,15 @@ bool rows16(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, i
          (H == 1 || st[1] % per == 0) && (T == 1 || st[2] % per == 0);
 }
 
-template <typename K>
+template <int W, typename K>
 int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int row_tiles) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * S));
-  cfg.blockDim = dim3(32 * kFewWarps);
+  cfg.blockDim = dim3(32 * W);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = cur_stream();
   cudaLaunchAttribute at[1];
@@ -1186,6 +1193,15 @@ int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int ro
     return set_error(BT_ECUDA, "bt_attention: launch failed: %s", cudaGetErrorString(e));
   }
   return BT_OK;
+}
+
+template <int W>
+int few_run(const AttnArgs& A, bool half, int64_t units, int S, int row_tiles) {
+  if (half)
+    return A.D <= 64 ? few_launch<W>(attn_few_kernel<64, W>, FewShape<64, kFewRows, W>::kSmem, A, units, S, row_tiles)
+                     : few_launch<W>(attn_few_kernel<128, W>, FewShape<128, kFewRows, W>::kSmem, A, units, S, row_tiles);
+  return A.D <= 64 ? few_launch<W>(attn_few32_kernel<64, W>, FewShape<64, kFewRows32, W>::kSmem, A, units, S, row_tiles)
+                   : few_launch<W>(attn_few32_kernel<128, W>, FewShape<128, kFewRows32, W>::kSmem, A, units, S, row_tiles);
 }
 
 // A tensor map over [B, H, T, D] (innermost D), 64 x 128 boxes; false where
@@ -1293,29 +1309,35 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   A.out = out->data;
   DevInfo di;
   if ((rc = dev_info(&di))) return rc;
-  // Few rows to a key head: straight from global memory, the keys split over
-  // a cluster until the GPU is full or a warp is down to four steps of 16.
   const bool half = q->dtype == BT_F16;
-  const int per = half ? 8 : 4;
-  const int64_t group = A.G * A.Tq;
-  if (A.Tk > 0 && group <= (half ? kFewMax : kFewMax32) && rows16(A.q, A.qs, A.B, A.H, A.Tq, D, per) &&
-      rows16(A.k, A.ks, A.B, Hk, A.Tk, D, per) && rows16(A.v, A.vs, A.B, Hk, A.Tk, D, per)) {
-    const int tile = half ? kFewRows : kFewRows32;
-    const int64_t row_tiles = (group + tile - 1) / tile, units = A.B * Hk * row_tiles;
+  const int per = half ? 8 : 4, few_rows = half ? kFewRows : kFewRows32;
+  const int64_t group = A.G * A.Tq, row_tiles = (group + few_rows - 1) / few_rows, units = A.B * Hk * row_tiles;
+  const bool pieces = rows16(A.q, A.qs, A.B, A.H, A.Tq, D, per) && rows16(A.k, A.ks, A.B, Hk, A.Tk, D, per) &&
+                      rows16(A.v, A.vs, A.B, Hk, A.Tk, D, per);
+  // The form with the least estimated time (us; measured with 1 to 64 batch
+  // entries, 1 to 16 heads, 32 to 1024 queries over 100 to 4096 keys): rows
+  // straight from global memory pay for every tile of rows and step of keys;
+  // the tiled forms for every round of CTAs and tile of keys.
+  //   float16, 1 x 1 head,   256 queries, 4096 keys of 64: 21 against 54 us
+  //            4 x 8 heads,  256 queries, 1000 keys of 64: 46 against 20 us
+  const double waves = ceil((double)(A.B * A.H * ((A.Tq + (half ? 2 * kTile : kRows32) - 1) / (half ? 2 * kTile : kRows32))) /
+                            di.sm_count);
+  const double few_us = half ? 17 + (double)units * (A.Tk / 16 + 1) * (D <= 64 ? 1.0e-3 : 3.0e-3)
+                             : 17 + (double)units * (A.Tk / 16 + 1) * (D <= 64 ? 1.6e-3 : 3.2e-3);
+  const double tile_us = half ? 9 + waves * (A.Tk / kTile + 1) * (D <= 64 ? 1.4 : 1.8)
+                              : 9 + waves * (A.Tk / kKeys32 + 1) * (D <= 64 ? 8.0 : 16.0);
+  if (A.Tk > 0 && pieces && (row_tiles == 1 || few_us < tile_us)) {
+    // the keys split over a cluster, then over more warps, until the GPU is
+    // full or a warp is down to four steps of 16 keys (32 x 16 heads, one
+    // query over 2000 keys: 54 us in 512 CTAs, 61 in 1024, 74 in 2048)
     int S = 1;
-    while (S < 8 && units * S < 4 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * kFewWarps * 64) S *= 2;
-    if (units * S < INT32_MAX) {
-      if (half)
-        return D <= 64 ? few_launch(attn_few_kernel<64>, FewShape<64, kFewRows>::kSmem, A, units, S, (int)row_tiles)
-                       : few_launch(attn_few_kernel<128>, FewShape<128, kFewRows>::kSmem, A, units, S, (int)row_tiles);
-      return D <= 64 ? few_launch(attn_few32_kernel<64>, FewShape<64, kFewRows32>::kSmem, A, units, S, (int)row_tiles)
-                     : few_launch(attn_few32_kernel<128>, FewShape<128, kFewRows32>::kSmem, A, units, S, (int)row_tiles);
-    }
+    while (S < 8 && units * S < 3 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * 4 * 64) S *= 2;
+    if (units * S < INT32_MAX)
+      return S == 8 && units * S < di.sm_count ? few_run<8>(A, half, units, S, (int)row_tiles)
+                                               : few_run<4>(A, half, units, S, (int)row_tiles);
   }
   if (!half && A.Tk > 0) {
     const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = A.B * A.H * q_tiles;
-    const bool pieces = rows16(A.q, A.qs, A.B, A.H, A.Tq, D, 4) && rows16(A.k, A.ks, A.B, Hk, A.Tk, D, 4) &&
-                        rows16(A.v, A.vs, A.B, Hk, A.Tk, D, 4);
     if (ctas < INT32_MAX && pieces)
       return D <= 64 ? attn_f32_launch<64, 4>(A, ctas, (int)q_tiles) : attn_f32_launch<128, 4>(A, ctas, (int)q_tiles);
     if (ctas < INT32_MAX)
