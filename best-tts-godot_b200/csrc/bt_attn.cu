@@ -157,8 +157,9 @@ struct AttnTc {
   AttnArgs a;
   int32_t q_mul[2], k_mul[2], v_mul[2];   // 0 where an axis (head, batch) is broadcast
   int32_t q_tiles;                        // items of a head
+  int32_t step_t, step_h, step_b;         // the grid's size in items, heads and batch entries
   uint32_t items;
-  int32_t wide;                           // out's rows: 32-, 16- or 2-byte stores
+  int32_t wide;                           // out: 2 by TMA stores, 1 rows of 16-byte pieces, 0 neither
 };
 
 template <int DP>
@@ -171,7 +172,8 @@ struct AttnShape {
   static constexpr int kP = kBeside ? 256 : 0;             // tensor memory: S at 0, 128
   static constexpr int kPStep = kBeside ? 64 : 128;
   static constexpr int kO = kBeside ? 384 : 256;
-  static constexpr int kSmem = 1024 + (2 + kSlots) * kRows + 512;
+  static constexpr bool kStage = DP == 64;                 // room for results on their way out
+  static constexpr int kSmem = 1024 + (2 + kSlots + (kStage ? 2 : 0)) * kRows + 512;
 };
 
 // The valid keys of a key tile as four words; all ones where every key is.
@@ -227,35 +229,53 @@ __device__ __forceinline__ uint32_t cvt_v(float2 x) {
   return h;
 }
 
-struct ItemPos {
-  int64_t b;
-  int h, t0;
-};
-__device__ __forceinline__ ItemPos item_pos(const AttnTc& A, uint32_t it) {
-  const uint32_t head = it / (uint32_t)A.q_tiles;
-  ItemPos p;
-  p.t0 = (int)(it - head * (uint32_t)A.q_tiles) * 2 * kTile;
-  p.b = head / (uint32_t)A.a.H;
-  p.h = (int)(head - (uint32_t)p.b * (uint32_t)A.a.H);
-  return p;
-}
+// The walk of a CTA over its items: item it is query tile pair t of head h of
+// batch entry b; the next one is gridDim.x on, in steps that the host has
+// split the same way, so that a step is three sums with carries.  The keys of
+// the next item are asked for an item ahead: the load's latency would stand
+// before each item.
+struct Items {
+  uint32_t it;
+  int t, h, b, n;
+  int t0;   // first query
+  __device__ __forceinline__ explicit Items(const AttnTc& A) : it(blockIdx.x) {
+    const uint32_t head = it / (uint32_t)A.q_tiles;
+    t = (int)(it - head * (uint32_t)A.q_tiles);
+    b = (int)(head / (uint32_t)A.a.H);
+    h = (int)(head - (uint32_t)b * (uint32_t)A.a.H);
+    n = (int)keys_of(A.a, b);   // (a CTA has an item)
+    t0 = t * 2 * kTile;
+    ask(A);
+  }
+  __device__ __forceinline__ bool live(const AttnTc& A) const { return it < A.items; }
+  __device__ __forceinline__ void next(const AttnTc& A) {
+    it += gridDim.x;
+    t = t2, h = h2, b = b2, n = n_next;
+    t0 = t * 2 * kTile;
+    ask(A);
+  }
 
-// The keys of an item's batch entry (0 past the last item), asked for an item
-// ahead by every role: the load's latency would stand before each item.
-__device__ __forceinline__ int item_keys(const AttnTc& A, uint32_t it) {
-  return it < A.items ? (int)keys_of(A.a, item_pos(A, it).b) : 0;
-}
+ private:
+  int t2, h2, b2, n_next;
+  __device__ __forceinline__ void ask(const AttnTc& A) {
+    t2 = t + A.step_t, h2 = h + A.step_h, b2 = b + A.step_b;
+    if (t2 >= A.q_tiles) t2 -= A.q_tiles, ++h2;
+    if (h2 >= (int)A.a.H) h2 -= (int)A.a.H, ++b2;
+    n_next = it + gridDim.x < A.items ? (int)keys_of(A.a, b2) : 0;
+  }
+};
 
 template <int DP>
 __global__ void __launch_bounds__(kAttnThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnTc A) {
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_out,
+                   const __grid_constant__ AttnTc A) {
   using Sh = AttnShape<DP>;
   extern __shared__ uint8_t smem_raw[];
   const unsigned base = (smem_u32(smem_raw) + 1023) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const unsigned ring = base + 2 * Sh::kRows;
-  uint64_t* bars = (uint64_t*)(smem + (2 + Sh::kSlots) * Sh::kRows);
+  uint64_t* bars = (uint64_t*)(smem + (2 + Sh::kSlots + (Sh::kStage ? 2 : 0)) * Sh::kRows);
   uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *s_free = bars + 6, *p_full = bars + 8;
   uint64_t* pv_done = bars + 10;   // [tile][key tile's parity]: two, so that a phase may pass unwaited for
   uint64_t *kv_full = bars + 14, *kv_empty = kv_full + Sh::kSlots, *v_ok = kv_empty + Sh::kSlots;
@@ -304,11 +324,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     auto your_turn = [&]() { asm volatile("bar.arrive %0, 256;\n" ::"r"(2 - tile) : "memory"); };
     if (tile == 1) your_turn();
     uint32_t g = 0;   // key tiles this query tile has worked on
-    int n_next = item_keys(A, blockIdx.x);
-    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
-      const ItemPos pos = item_pos(A, it);
-      const int n = n_next;
-      n_next = item_keys(A, it + gridDim.x);
+    for (Items pos(A); pos.live(A); pos.next(A)) {
+      const int n = pos.n;
       const int64_t t = pos.t0 + tile * kTile + (warp & 3) * 32 + lane;
       if (pos.t0 + tile * kTile >= a.Tq) continue;
       const bool turns = pos.t0 + kTile < a.Tq;   // both tiles have work
@@ -451,9 +468,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                                         : __floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
           y[j] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        if (t < a.Tq) {
+        if (Sh::kStage && A.wide == 2) {
+          // a row of 128 bytes, its 16-byte pieces where the store's swizzle
+          // has them
+          const int row = (warp & 3) * 32 + lane;
+          if (i == 0) {   // (the last item's store has read the tile: its issuer waited, all wait for the issuer)
+            if (row == 0) bulk_wait_read<0>();
+            asm volatile("bar.sync %0, 128;\n" ::"r"(3 + tile) : "memory");
+          }
+          uint8_t* at = smem + (2 + Sh::kSlots + tile) * Sh::kRows + row * 128;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(at + (((4 * i + j) ^ (row & 7)) << 4)) =
+                make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+        } else if (t < a.Tq) {
           const int left = a.D - 32 * i;
-          if (A.wide == 16) {
+          if (A.wide) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (8 * j < left)
@@ -464,6 +494,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             for (int j = 0; j < 32; ++j)
               if (j < left) out[(int64_t)(32 * i + j) * a.os[3]] = e[j];
           }
+        }
+      }
+      if (Sh::kStage && A.wide == 2) {
+        fence_async_shared();
+        asm volatile("bar.sync %0, 128;\n" ::"r"(3 + tile) : "memory");
+        if ((warp & 3) == 0 && lane == 0) {
+          tma_store4(&map_out, base + (2 + Sh::kSlots + tile) * Sh::kRows, 0, pos.t0 + tile * kTile, pos.h, pos.b);
+          bulk_commit();
         }
       }
       tc_fence_before();   // (O is read before this warp's next arrival lets it be written)
@@ -505,11 +543,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       __syncwarp();
       ++g;
     };
-    int n_next = item_keys(A, blockIdx.x);
-    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
-      const ItemPos pos = item_pos(A, it);
-      const int nb = (n_next + kTile - 1) / kTile;
-      n_next = item_keys(A, it + gridDim.x);
+    for (Items pos(A); pos.live(A); pos.next(A)) {
+      const int nb = (pos.n + kTile - 1) / kTile;
       if (pos.t0 + i * kTile >= a.Tq) {   // no such tile in this item: pass its keys on
         for (int j = 0; j < 2 * nb; ++j, ++r) {
           tc_wait(kv_full + r % Sh::kSlots, r / Sh::kSlots & 1, aborted);
@@ -541,13 +576,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     if (lane == 0) {
       unsigned q_ph[2] = {1, 1};
       uint32_t g = 0;
-      int n_next = item_keys(A, blockIdx.x);
-      for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
-        const ItemPos pos = item_pos(A, it);
-        const int nb = (n_next + kTile - 1) / kTile;
-        n_next = item_keys(A, it + gridDim.x);
+      for (Items pos(A); pos.live(A); pos.next(A)) {
+        const int nb = (pos.n + kTile - 1) / kTile;
         if (nb == 0) continue;
-        const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1, b = (int)pos.b, hk = pos.h / (int)a.G;
+        const int tiles = pos.t0 + kTile < a.Tq ? 2 : 1, b = pos.b, hk = pos.h / (int)a.G;
         auto load = [&](const CUtensorMap* m, unsigned dst, uint64_t* bar, int t0, int h, int bb) {
           mbar_arrive_expect_tx(bar, Sh::kRows);
 #pragma unroll
@@ -573,11 +605,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp == 11 && fix_v) {
     uint32_t g = 1;
-    int n_next = item_keys(A, blockIdx.x);
-    for (uint32_t it = blockIdx.x; it < A.items; it += gridDim.x) {
-      const ItemPos pos = item_pos(A, it);
-      const int n = n_next;
-      n_next = item_keys(A, it + gridDim.x);
+    for (Items pos(A); pos.live(A); pos.next(A)) {
+      const int n = pos.n;
       const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
       for (int k0 = 0; k0 < n; k0 += kTile, g += 2) {
         bool in[4];
@@ -613,6 +642,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
     }
   }
+  if (Sh::kStage && warp < 8 && (warp & 3) == 0 && lane == 0) bulk_wait_all();
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -1229,13 +1259,17 @@ bool attn_map(CUtensorMap* m, const void* p, const int64_t* st, int64_t B, int64
 }
 
 template <int DP>
-int attn_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnTc& A, int sms) {
+int attn_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, AttnTc& A,
+                   int sms) {
   auto kern = attn_tc_kernel<DP>;
   constexpr int smem = AttnShape<DP>::kSmem;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
   const int grid = (int)(A.items < (uint32_t)sms ? A.items : (uint32_t)sms);
-  kern<<<grid, kAttnThreads, smem, cur_stream()>>>(mq, mk, mv, A);
+  A.step_t = grid % A.q_tiles;
+  A.step_h = grid / A.q_tiles % (int)A.a.H;
+  A.step_b = grid / A.q_tiles / (int)A.a.H;
+  kern<<<grid, kAttnThreads, smem, cur_stream()>>>(mq, mk, mv, mo, A);
   return check_launch("bt_attention");
 }
 
@@ -1352,10 +1386,15 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
       P.a = A;
       P.q_tiles = (int32_t)q_tiles;
       P.items = (uint32_t)items;
-      const bool rows16 = ((uintptr_t)A.out & 15) == 0 && D % 8 == 0 && A.os[3] == 1 && A.os[0] % 8 == 0 && A.os[1] % 8 == 0 &&
-                          A.os[2] % 8 == 0;
-      P.wide = rows16 ? 16 : 2;
-      return D <= 64 ? attn_tc_launch<64>(mq, mk, mv, P, di.sm_count) : attn_tc_launch<128>(mq, mk, mv, P, di.sm_count);
+      CUtensorMap mo = {};
+      int32_t o_mul[2];
+      // (a TMA store needs every axis of its own: no two rows of out overlap)
+      P.wide = !rows16(A.out, A.os, A.B, A.H, A.Tq, D, 8) ? 0
+               : attn_map(&mo, A.out, A.os, A.B, A.H, A.Tq, D, o_mul, &rc) && (A.B == 1 || o_mul[1]) && (A.H == 1 || o_mul[0])
+                   ? 2
+                   : 1;
+      if (rc) return rc;
+      return D <= 64 ? attn_tc_launch<64>(mq, mk, mv, mo, P, di.sm_count) : attn_tc_launch<128>(mq, mk, mv, mo, P, di.sm_count);
     }
     if (rc) return rc;
   }

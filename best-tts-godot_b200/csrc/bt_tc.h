@@ -92,11 +92,11 @@ __device__ __forceinline__ void tma_load4(unsigned dst, const CUtensorMap* m, un
       : "memory");
 }
 
-// Shared memory -> the box at (x, y), clipped to the map's extents, in this
-// thread's current bulk group.
-__device__ __forceinline__ void tma_store2(const CUtensorMap* m, unsigned src, int x, int y) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(m), "r"(src), "r"(x),
-               "r"(y)
+// Shared memory -> the box at (x, y, z, w), clipped to the map's extents, in
+// this thread's current bulk group.
+__device__ __forceinline__ void tma_store4(const CUtensorMap* m, unsigned src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n" ::"l"(m), "r"(src),
+               "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
 // Until at most N of this thread's bulk groups still read shared memory.
