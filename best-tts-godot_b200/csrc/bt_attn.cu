@@ -125,20 +125,26 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // for each tile the 128 x 128 float32 scores S of the current key tile, the
 // float16 weights P (D <= 64: beside S; else over S) and the 128 x D output O.
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a query row, reads its
-//                   128 scores into registers, writes its weights
+//                   128 scores into registers (216 of them: the other warps
+//                   give theirs up), writes its weights
 //   warps 8, 9      issue tile 0's, 1's S = Q K^T and O += P V (P read from
-//                   tensor memory); one warp for both was the bottleneck: its
-//                   waits and commits alone took 2000 clocks a key tile
+//                   tensor memory)
 //   warp 10         TMA loads: the item's Q tiles, a ring of K and V tiles
 //   warp 11         zeroes the rows of V whose keys take no part (only where
 //                   there are lengths or a mask: a weight of 0 times NaN
 //                   would not be 0)
-// The two tiles take turns: while one's softmax runs, the tensor cores work
-// for the other; with P beside S the next scores are also computed while the
-// softmax still works on these.  (Blocks of 64 keys with two score buffers a
-// tile measured slower, 655 against 536 us at 16 heads of 8192 x 8192 x 64:
-// the softmax is bound by its instructions' latencies, and each block has a
-// fixed part of about 700 clocks.)
+// With P beside S the next scores are computed while the softmax still works
+// on these; else the tiles overlap each other.  The softmax bounds it: its
+// exponentials alone take 1024 clocks a 128 x 128 tile, the tensor cores 512
+// (D = 64) or 1024 (D = 128), and with two warps a scheduler the latencies
+// between them show.  So tile 0 and 1 take turns at the exponentials (each
+// then has the special-function unit to itself while the other waits, reads
+// and compares: 134 -> 120 us at 16 heads of 4096 x 4096 x 64).  There, and at
+// D = 128, 120 and 151 us are 575 and 909 TFLOP/s.  Measured and not taken:
+// blocks of 64 keys with two score buffers a tile (174 us: each block has a
+// fixed part), two threads a row (144 us), scores read twice instead of kept
+// (157 us), the maximum found along with the weights and these redone where it
+// grew (162 us).
 //
 // Softmax: with c = scale log2(e) and a reference value m per row,
 // p = 2^(s c - m c + 7).  m is the row's running maximum, but it moves (and O
@@ -151,7 +157,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 constexpr int kTile = 128;
 constexpr int kAttnThreads = 384;
 constexpr float kGrow = 8.0f, kLift = 7.0f;
-constexpr int kPolyOf8 = 0;   // of eight pairs of weights, those on the FMA pipe
 
 struct AttnTc {
   AttnArgs a;
@@ -193,24 +198,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-
-// 2^x of two values on the FMA pipe (the special-function unit gives four
-// exponentials a clock and scheduler, and bounds this softmax): x = n + f with
-// n = rint(x) from the sum with 1.5 2^23, 2^f by a polynomial of degree 4 on
-// [-1/2, 1/2] (minimax by exchange, relative error 2.6e-6), n added to the
-// exponent.  x <= 16; below -126 gives 2^-126.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 t = pk_add(x, pk(12582912.0f));
-  const float2 f = pk_fma(pk_add(t, pk(-12582912.0f)), pk(-1.0f), x);
-  float2 p = pk_fma(pk(0.009570101911165427f), f, pk(0.055917860319388245f));
-  p = pk_fma(p, f, pk(0.2402474482786378f));
-  p = pk_fma(p, f, pk(0.6931218147366892f));
-  p = pk_fma(p, f, pk(0.9999992614457122f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // The same operations where they are written: the order is the schedule.
@@ -411,18 +398,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         // Pair x is scaled in step x, exponentiated in step x + 1, summed and
         // rounded in step x + 3, in this order (volatile): the special-function
         // unit takes eight clocks an instruction, and what is issued between
-        // two of its instructions is free.
+        // two of its instructions is free.  (A quarter of the exponentials as
+        // polynomials on the FMA pipe instead measured slower: 126 against
+        // 120 us at 16 heads of 4096 x 4096 x 64.)
         float2 e[64];
         uint32_t p[4][16];
 #pragma unroll
         for (int x = 0; x < 64 + 3; ++x) {
           if (x < 64)
             e[x] = pk_fma_v(make_float2(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, mc2);
-          const bool poly = x >= 1 && x <= 64 && (x - 1) % 8 >= 8 - kPolyOf8;
-          if (x >= 1 && x <= 64 && !poly) ex2_v(e[x - 1].x);
+          if (x >= 1 && x <= 64) ex2_v(e[x - 1].x);
           if (x >= 3) part_l[x & 1] = pk_add(part_l[x & 1], e[x - 3]);
-          if (x >= 1 && x <= 64 && !poly) ex2_v(e[x - 1].y);
-          if (poly) e[x - 1] = exp2_poly(e[x - 1]);
+          if (x >= 1 && x <= 64) ex2_v(e[x - 1].y);
           if (x >= 3) {
             const int y = x - 3;
             p[y / 16][y % 16] = cvt_v(e[y]);
@@ -1027,6 +1014,10 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
 // rows.  K and V tiles arrive by cp.async (16 bytes, or 4 for any strides;
 // rows of keys that take no part are filled with zeros), for dims up to 64
 // the next tile while this one is worked on.  Bound by the FMA pipe.
+// Measured: 37 TFLOP/s at 8 x 16 heads of 1024 x 1024 x 64, half of the FMA
+// pipe's rate, and 168 us at 8 x 12 heads of up to 510 x 510 x 64 (three rounds
+// of CTAs); 8 x 8 sums a thread with two CTAs of 128 threads on an SM came to
+// the same (36 TFLOP/s, 175 us).
 constexpr int kRows32 = 128, kKeys32 = 64, kThreads32 = 256;
 
 template <int DP>
@@ -1189,8 +1180,8 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
 template <int DP, int N>
 int attn_f32_launch(const AttnArgs& A, int64_t ctas, int q_tiles) {
   auto kern = attn_f32_kernel<DP, N>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape32<DP>::kSmem);
-  if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  static bool raised[64];
+  if (const int rc = raise_smem(kern, Shape32<DP>::kSmem, raised)) return rc;
   kern<<<(unsigned)ctas, kThreads32, Shape32<DP>::kSmem, cur_stream()>>>(A, q_tiles);
   return check_launch("bt_attention");
 }
@@ -1201,11 +1192,23 @@ bool rows16(const void* p, const int64_t* st, int64_t B, int64_t H, int64_t T, i
          (H == 1 || st[1] % per == 0) && (T == 1 || st[2] % per == 0);
 }
 
+// Raises a kernel's shared-memory limit, once per device.
+template <typename K>
+int raise_smem(K kern, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+  }
+  return e == cudaSuccess ? BT_OK : set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+}
+
 template <int W, typename K>
 int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int row_tiles) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  if (smem > 48 * 1024) {   // (float16, dims above 64, eight warps: the one such kernel)
+    static bool raised[64];
+    if (const int rc = raise_smem(kern, smem, raised)) return rc;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * S));
@@ -1263,8 +1266,8 @@ int attn_tc_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorM
                    int sms) {
   auto kern = attn_tc_kernel<DP>;
   constexpr int smem = AttnShape<DP>::kSmem;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
+  static bool raised[64];
+  if (const int rc = raise_smem(kern, smem, raised)) return rc;
   const int grid = (int)(A.items < (uint32_t)sms ? A.items : (uint32_t)sms);
   A.step_t = grid % A.q_tiles;
   A.step_h = grid / A.q_tiles % (int)A.a.H;

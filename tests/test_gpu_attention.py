@@ -44,6 +44,55 @@ def test_sizes(gpu_runtime, B, H, Hk, Tq, Tk, D, dtype):
         assert layout == "head" or o.permute(0, 2, 1, 3).is_contiguous()
 
 
+# (batch, heads, queries, keys, dim): enough heads and queries that the tiled
+# forms run, with more items than the GPU has SMs, a second query tile of a few
+# rows or none, and key tiles that wrap the ring of tiles
+MANY = [(40, 8, 130, 260, 64), (40, 8, 130, 260, 128), (25, 12, 100, 600, 64), (25, 12, 100, 600, 40), (20, 10, 300, 1500, 96),
+        (10, 16, 513, 1000, 64), (9, 20, 257, 129, 128), (3, 64, 128, 2100, 64)]
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("B,H,Tq,Tk,D", MANY)
+def test_many_items(gpu_runtime, B, H, Tq, Tk, D, dtype):
+    g = torch.Generator("cuda").manual_seed(B + Tk)
+    q, k, v = (_states(g, B, h, t, D, dtype, "token") for h, t in ((H, Tq), (H // 2, Tk), (H // 2, Tk)))
+    lengths = torch.randint(0, Tk + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[1], lengths[2], lengths[B - 1] = 0, Tk, 0
+    mask = torch.rand(B, Tk, generator=g, device="cuda") < 0.8
+    mask[0, :128] = False
+    _run(gpu_runtime, q, k, v, "all")
+    _run(gpu_runtime, q, k, v, "lengths", lengths=lengths)
+    _run(gpu_runtime, q, k, v, "mask", key_mask=mask)
+    o = _run(gpu_runtime, q, k, v, "both", key_mask=mask, lengths=lengths)
+    out = ~(mask & (torch.arange(Tk, device="cuda") < lengths[:, None]))
+    k2, v2 = (t.masked_fill(out[:, None, :, None], float("nan")) for t in (k, v))
+    assert torch.equal(gpu_runtime.attention(q, k2, v2, key_mask=mask, lengths=lengths), o)
+    for _ in range(3):
+        assert torch.equal(gpu_runtime.attention(q, k, v, key_mask=mask, lengths=lengths), o)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_items_growing_and_non_finite(gpu_runtime, D, dtype):
+    """Rows whose reference moves in every key tile, beside rows where it never
+    does; NaN and infinite scores in some rows of the tiled forms."""
+    rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(D)
+    B, H, Tq, Tk = 6, 30, 300, 900
+    q, k, v = (_states(g, B, H, t, D, dtype) for t in (Tq, Tk, Tk))
+    ramp = torch.linspace(0, 60, Tk, device="cuda")
+    k[..., 0] = ramp.to(dtype)
+    q[..., 0] = torch.where(torch.rand(B, H, Tq, generator=g, device="cuda") < 0.3, 30.0, 0.1).to(dtype)
+    o = _run(rt, q, k, v, "ramp")
+    q2, k2 = q.clone(), k.clone()
+    q2[0, 0, 5, 3] = float("nan")
+    q2[1, 2, 299, 0] = float("inf")
+    k2[2, 3, 700, 1] = float("nan")      # every row of head (2, 3)
+    o2 = rt.attention(q2, k2, v)
+    assert o2[0, 0, 5].isnan().all() and o2[1, 2, 299].isnan().all() and o2[2, 3].isnan().all()
+    o2[0, 0, 5], o2[1, 2, 299], o2[2, 3] = o[0, 0, 5], o[1, 2, 299], o[2, 3]
+    assert torch.equal(o2, o)
+
+
 @pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("Tq", [1, 6, 130, 400])
 def test_lengths_and_masks(gpu_runtime, Tq, dtype):
@@ -207,19 +256,19 @@ def test_rows_around_the_result_are_left_alone(gpu_runtime):
     from bt_b200._lib import check
     from bt_b200.runtime import tensor_desc
     rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(4)
-    for dtype in (F16, F32):
-        for Tq in (1, 130, 300):
-            q, k, v = (_states(g, 2, 2, t, 64, dtype) for t in (Tq, 90, 90))
-            room = torch.full((2, 4, Tq + 5, 80), 7.0, dtype=dtype, device="cuda")
-            out = room[:, 1:3, 2:2 + Tq, 8:72]
-            rt._stream()
-            check(rt.lib.bt_attention(ctypes.byref(tensor_desc(q)), ctypes.byref(tensor_desc(k)), ctypes.byref(tensor_desc(v)),
-                                      None, None, 0.125, ctypes.byref(tensor_desc(out))), "bt_attention")
-            torch.cuda.synchronize()
-            assert torch.equal(out, rt.attention(q, k, v))
-            rest = room.clone()
-            rest[:, 1:3, 2:2 + Tq, 8:72] = 7.0
-            assert (rest == 7.0).all()
+    for dtype, Tq, D, left, wide in ((dt, t, d, left, wide) for dt in (F16, F32) for t in (1, 130, 300)
+                                     for d in (64, 128, 40) for left, wide in ((8, 144), (3, 141), (1, 144))):
+        q, k, v = (_states(g, 2, 16, t, D, dtype) for t in (Tq, 90, 90))
+        room = torch.full((2, 18, Tq + 5, wide), 7.0, dtype=dtype, device="cuda")
+        out = room[:, 1:17, 2:2 + Tq, left:left + D]
+        rt._stream()
+        check(rt.lib.bt_attention(ctypes.byref(tensor_desc(q)), ctypes.byref(tensor_desc(k)), ctypes.byref(tensor_desc(v)),
+                                  None, None, 0.125, ctypes.byref(tensor_desc(out))), "bt_attention")
+        torch.cuda.synchronize()
+        assert torch.equal(out, rt.attention(q, k, v, scale=0.125))
+        rest = room.clone()
+        rest[:, 1:17, 2:2 + Tq, left:left + D] = 7.0
+        assert (rest == 7.0).all()
 
 
 def test_repeats_bit_for_bit_on_streams_threads_and_graphs(gpu_runtime):
@@ -291,3 +340,12 @@ def test_attention_block(gpu_runtime, T, S):
         o = _run(rt, *heads, "block", lengths=lengths)
         y = project(o.permute(0, 2, 1, 3).reshape(B, T, C), wo)
         assert y.shape == (B, T, C) and torch.isfinite(y).all()
+
+
+def test_no_wait_gave_up(gpu_runtime):
+    """Every bounded wait of the runs above ended by what it waited for."""
+    import ctypes
+    from bt_b200._lib import check
+    n = ctypes.c_uint32(99)
+    check(gpu_runtime.lib.bt_wait_timeouts(ctypes.byref(n)), "bt_wait_timeouts")
+    assert n.value == 0
