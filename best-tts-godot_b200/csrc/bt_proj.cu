@@ -251,6 +251,20 @@ __device__ __forceinline__ void mm_store(TO* p, float v) {
   else *p = v;
 }
 
+// Two values of neighbouring tokens, rounded to float16 as a pair (two clocks
+// a warp; one value alone takes eight).
+template <typename TO>
+__device__ __forceinline__ void mm_store2(TO* p, TO* q, float v, float w) {
+  if constexpr (sizeof(TO) == 2) {
+    const __half2 h = __floats2half2_rn(v, w);
+    *p = __low2half(h);
+    *q = __high2half(h);
+  } else {
+    *p = v;
+    *q = w;
+  }
+}
+
 // kChunk columns of an accumulator.
 template <int kChunk>
 __device__ __forceinline__ void mm_ld(uint32_t at, uint32_t (&r)[kChunk]) {
@@ -450,7 +464,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) matmul_tc_kernel(const __grid_c
         if (c0 + kChunk <= cols) {
           if (live) {
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j, op += A.ldo) mm_store(op, y[j]);
+            for (int j = 0; j < kChunk; j += 2, op += 2 * A.ldo) mm_store2(op, op + A.ldo, y[j], y[j + 1]);
           }
         } else {
 #pragma unroll
@@ -577,39 +591,53 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
   return BT_OK;
 }
 
-template <typename TO>
-int mm_run(const MmArgs& A, int sms, const char* what) {
-  // The tile and the split with the least estimated time, in SM clocks: a
-  // block of 128 along the summed axis takes the longer of its matrix
-  // instructions (8192 products a clock) and its loads (64 bytes a clock);
-  // a tile adds its stores, a launch its start, a split its exchange.
-  const int kblocks = (int)((A.K + 127) / 128);
-  int best_nt = 0, best_cg = 1, best_s = 1;
+// The tile and the split with the least estimated time, in SM clocks: a block
+// of 128 along the summed axis takes the longer of its matrix instructions
+// (8192 products a clock) and its loads (64 bytes a clock); a tile adds its
+// stores, a launch its start, a split its exchange.
+struct MmChoice {
+  int64_t M, N, K;
+  int sms, nt, cg, split;
+};
+
+void mm_choose(MmChoice& c) {
+  const int kblocks = (int)((c.K + 127) / 128);
   double best = 1e300;
   auto consider = [&](int nt, int cg, int s) {
-    const double tiles = (double)((A.N + 128 * cg - 1) / (128 * cg)) * (double)((A.M + nt - 1) / nt);
-    const double units = cg == 2 ? sms / 2 : sms / s;
+    const double tiles = (double)((c.N + 128 * cg - 1) / (128 * cg)) * (double)((c.M + nt - 1) / nt);
+    const double units = cg == 2 ? c.sms / 2 : c.sms / s;
     const double waves = ceil(tiles / units);
     const double mma = 2.0 * nt, load = (16384 + nt * 128 / cg) / 64.0;
     const double per = ceil((double)kblocks / s) * (mma > load ? mma : load);
     const double store = nt * 8.0;
     const double t = 3000 + waves * (per > store ? per : store) + store + (s > 1 ? 2500 + 20.0 * nt : 0);
-    if (t < best) best = t, best_nt = nt, best_cg = cg, best_s = s;
+    if (t < best) best = t, c.nt = nt, c.cg = cg, c.split = s;
   };
   for (int nt = 16; nt <= 256; nt *= 2) {
-    if (nt > 16 && A.M <= nt / 2) break;
+    if (nt > 16 && c.M <= nt / 2) break;
     consider(nt, 1, 1);
     if (nt <= 128)
       for (int s = 2; s <= 8 && s <= kblocks; ++s) consider(nt, 1, s);
   }
   consider(256, 2, 1);
-  if (best_cg == 2) return mm_launch<256, 2, TO>(A, 1, sms, what);
-  switch (best_nt) {
-    case 16: return mm_launch<16, 1, TO>(A, best_s, sms, what);
-    case 32: return mm_launch<32, 1, TO>(A, best_s, sms, what);
-    case 64: return mm_launch<64, 1, TO>(A, best_s, sms, what);
-    case 128: return mm_launch<128, 1, TO>(A, best_s, sms, what);
-    default: return mm_launch<256, 1, TO>(A, best_s, sms, what);
+}
+
+template <typename TO>
+int mm_run(const MmArgs& A, int sms, const char* what) {
+  // (a thread's products mostly repeat a few sizes)
+  static thread_local MmChoice seen[8] = {};
+  MmChoice& c = seen[(A.M * 31 + A.N * 7 + A.K) & 7];
+  if (c.M != A.M || c.N != A.N || c.K != A.K || c.sms != sms) {
+    c.M = A.M, c.N = A.N, c.K = A.K, c.sms = sms;
+    mm_choose(c);
+  }
+  if (c.cg == 2) return mm_launch<256, 2, TO>(A, 1, sms, what);
+  switch (c.nt) {
+    case 16: return mm_launch<16, 1, TO>(A, c.split, sms, what);
+    case 32: return mm_launch<32, 1, TO>(A, c.split, sms, what);
+    case 64: return mm_launch<64, 1, TO>(A, c.split, sms, what);
+    case 128: return mm_launch<128, 1, TO>(A, c.split, sms, what);
+    default: return mm_launch<256, 1, TO>(A, c.split, sms, what);
   }
 }
 
