@@ -595,35 +595,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     for (Items pos(A); pos.live(A); pos.next(A)) {
       const int n = pos.n;
       const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
-      for (int k0 = 0; k0 < n; k0 += kTile, g += 2) {
-        bool in[4];
+      // which of this lane's four rows of a key tile take no part
+      auto look = [&](int k0) {
+        unsigned out = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int k = k0 + 32 * i + lane;
-          in[i] = k < n && (!mask || mask[(int64_t)k * a.mask_sk]);
+          if (!(k < n && (!mask || mask[(int64_t)k * a.mask_sk]))) out |= 1u << i;
         }
+        return out;
+      };
+      unsigned next = look(0);
+      for (int k0 = 0; k0 < n; k0 += kTile, g += 2) {
+        const unsigned out = next;
+        next = look(k0 + kTile);
         const int sl = (int)(g % Sh::kSlots);
         tc_wait(kv_full + sl, g / Sh::kSlots & 1, aborted);
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          unsigned out = ~__ballot_sync(0xffffffffu, in[i]);
-          any |= out != 0;
-          // eight lanes clear a 128-byte row, four rows at a time
-          for (; out; ) {
-            unsigned pick = out;   // the (lane / 8)-th of the rows still to clear
-            for (int y = 0; y < (lane >> 3); ++y) pick &= pick - 1;
-            if (pick) {
-              const int row = 32 * i + __ffs(pick) - 1;
+        if (__any_sync(0xffffffffu, out != 0)) {
+          // a lane clears its row's 128 bytes piece by piece, each lane
+          // beginning at another one, so that no two meet in a bank
+          uint8_t* at = smem + (2 + sl) * Sh::kRows + lane * 128;
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i, at += 32 * 128)
+            if (out >> i & 1) {
 #pragma unroll
               for (int x = 0; x < Sh::kPanels; ++x)
-                *reinterpret_cast<uint4*>(smem + (2 + sl) * Sh::kRows + x * Sh::kPanel + row * 128 + (lane & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                  *reinterpret_cast<uint4*>(at + x * Sh::kPanel + ((y + lane & 7) << 4)) = make_uint4(0, 0, 0, 0);
             }
-            for (int y = 0; y < 4; ++y) out &= out - 1;
-          }
+          fence_async_shared();
         }
-        if (any) fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_ok + sl);
       }
