@@ -645,9 +645,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // ---- few queries ---------------------------------------------------------------
 // A step of generation: the queries that share a key head (Tq of each of its
 // G query heads) are rows of one or a few 16-row tiles, and the time is that
-// of reading K and V once.  A warp takes 16 keys at a time, straight from
-// global memory into the operands of 16 x 8 x 16 products (far below the
-// tensor cores' rate here, and free of shared memory):
+// of reading K and V once.  A warp takes 16 keys at a time, fetched three
+// steps deep into a ring of its own (cp.async), as operands of 16 x 8 x 16
+// products (far below the tensor cores' rate here):
 //   S = Q K^T  the order of the summed dims is free, so a lane's 16 bytes of a
 //              key row are dims 8c..8c+7 of two products, Q permuted alike;
 //   O += P V   a lane holds dims 8q..8q+7 of the four keys its weights belong
@@ -673,6 +673,10 @@ struct FewShape {
   static constexpr int kPitch = DP + 4;
   static constexpr int kPart = ROWS * kPitch;                 // floats
   static constexpr int kSmem = W * kPart * 4;
+  // the float16 form's ring: 16 rows of K, then of V, for each step; the parts
+  // lie over it at the end
+  static constexpr int kSteps = 3, kRow = DP * 2, kStep = 2 * 16 * kRow;
+  static constexpr int kRing = W * kSteps * kStep;
 };
 
 // Joins the parts of all warps of the CTA, or of the cluster (each CTA then
@@ -727,7 +731,7 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
 template <int DP, int W>
 __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
   using Sh = FewShape<DP, kFewRows, W>;
-  extern __shared__ float few_sm[];
+  extern __shared__ __align__(16) float few_sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = lane >> 2, c = lane & 3;
   const unsigned part = S > 1 ? cluster_rank() : 0;
   uint32_t u = blockIdx.x / (unsigned)S;
@@ -763,28 +767,48 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
   // this CTA's keys: whole steps of 16, as even as they go
   const int steps = (n + 15) / 16;
   const int s0 = (int)((int64_t)steps * part / S), s1 = (int)((int64_t)steps * (part + 1) / S);
-  uint4 kr[2][DP / 32], vr[4][DP / 64];
-  auto load_k = [&](int k0) {
+  // the ring: a row's 16-byte pieces are permuted so that the reads below meet
+  // no bank twice (K: eight lanes read four pieces of two neighbouring rows;
+  // V: two pieces of every other row)
+  const unsigned ring = smem_u32(few_sm) + warp * (Sh::kSteps * Sh::kStep);
+  auto fetch = [&](int st, int slot) {
+    if (st < s1) {
+      constexpr int kPieces = DP / 8;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int key = k0 + 8 * h + q;
+      for (int i = 0; i < 16 * kPieces / 32; ++i) {
+        const int piece = lane + 32 * i, row = piece / kPieces, ch = piece % kPieces, key = 16 * st + row;
+        const int bytes = key < n && 8 * ch < A.D ? 16 : 0;
+        const int64_t ko = bytes ? key * A.ks[2] + 8 * ch : 0, vo = bytes ? key * A.vs[2] + 8 * ch : 0;
+        const unsigned at = ring + slot * Sh::kStep + row * Sh::kRow;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(at + ((ch ^ ((row & 1) << 2 | (row >> 1 & 3))) << 4)),
+                     "l"(kp + ko), "r"(bytes)
+                     : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(at + 16 * Sh::kRow + ((ch ^ (row & 7)) << 4)),
+                     "l"(vp + vo), "r"(bytes)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+  auto piece = [&](unsigned at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+  };
+#pragma unroll
+  for (int i = 0; i < Sh::kSteps - 1; ++i) fetch(s0 + warp + i * W, i);
+  for (int st = s0 + warp, slot = 0; st < s1; st += W, slot = slot + 1 == Sh::kSteps ? 0 : slot + 1) {
+    const int k0 = 16 * st;
+    fetch(st + (Sh::kSteps - 1) * W, slot == 0 ? Sh::kSteps - 1 : slot - 1);
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(Sh::kSteps - 1) : "memory");
+    __syncwarp();
+    const unsigned kt = ring + slot * Sh::kStep, vt = kt + 16 * Sh::kRow;
+    uint4 kr[2][DP / 32], vr[4][DP / 64];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int x = 0; x < DP / 32; ++x)
-        kr[h][x] = key < n && 32 * x + 8 * c < A.D ? __ldg(reinterpret_cast<const uint4*>(kp + key * A.ks[2] + 32 * x + 8 * c))
-                                                   : make_uint4(0, 0, 0, 0);
-    }
-  };
-  if (s0 + warp < s1) load_k(16 * (s0 + warp));
-  for (int st = s0 + warp; st < s1; st += W) {
-    const int k0 = 16 * st;
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int key = k0 + 2 * c + (y & 1) + 8 * (y >> 1);
-#pragma unroll
-      for (int x = 0; x < DP / 64; ++x)
-        vr[y][x] = key < n && 64 * x + 8 * q < A.D ? __ldg(reinterpret_cast<const uint4*>(vp + key * A.vs[2] + 64 * x + 8 * q))
-                                                   : make_uint4(0, 0, 0, 0);
-    }
+        kr[h][x] = piece(kt + (8 * h + q) * Sh::kRow + (((4 * x + c) ^ ((q & 1) << 2 | (q >> 1 & 3))) << 4));
     bool in[4] = {true, true, true, true};   // keys 2 c, 2 c + 1 of each eight
     if (mask || k0 + 16 > n) {
 #pragma unroll
@@ -801,8 +825,13 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
         mma_16x8x16(s[h], qa[2 * x], kr[h][x].x, kr[h][x].y);
         mma_16x8x16(s[h], qa[2 * x + 1], kr[h][x].z, kr[h][x].w);
       }
-    // the next step's keys, while this one's weights are computed
-    if (st + W < s1) load_k(16 * (st + W));
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int row = 2 * c + (y & 1) + 8 * (y >> 1);
+#pragma unroll
+      for (int x = 0; x < DP / 64; ++x) vr[y][x] = piece(vt + row * Sh::kRow + (((8 * x + q) ^ (row & 7)) << 4));
+    }
+    __syncwarp();   // (the step is read: its place may be filled)
     // scores of rows q (s[.][0, 1]) and q + 8 (s[.][2, 3]), keys 2 c, 2 c + 1 of each eight
     if (mask || k0 + 16 > n) {
 #pragma unroll
@@ -861,6 +890,8 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
   }
+  asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+  __syncthreads();   // every warp is done with its ring
   // the warp's part: O[row][dim], then the maximum and the sum.  Column 2 c + e
   // of 8-column tile 8 x + j is dim 64 x + 8 (2 c + e) + j.
   float* mine = few_sm + warp * Sh::kPart;
@@ -886,7 +917,7 @@ template <int DP, int W>
 __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constant__ AttnArgs A, int S, int row_tiles) {
   using Sh = FewShape<DP, kFewRows32, W>;
   constexpr int R = kFewRows32, Y = DP / 32, kAhead = DP == 64 ? 4 : 2;   // steps of four keys loaded together
-  extern __shared__ float few_sm[];
+  extern __shared__ __align__(16) float few_sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, x = lane & 7, grp = lane >> 3;
   const unsigned part = S > 1 ? cluster_rank() : 0;
   uint32_t u = blockIdx.x / (unsigned)S;
@@ -1206,9 +1237,9 @@ int raise_smem(K kern, int bytes, bool (&done)[64]) {
   return e == cudaSuccess ? BT_OK : set_error(BT_ECUDA, "bt_attention: shared memory: %s", cudaGetErrorString(e));
 }
 
-template <int W, typename K>
-int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int row_tiles) {
-  if (smem > 48 * 1024) {   // (float16, dims above 64, eight warps: the one such kernel)
+template <int W, auto kern>
+int few_launch(int smem, const AttnArgs& A, int64_t units, int S, int row_tiles) {
+  if (smem > 48 * 1024) {
     static bool raised[64];
     if (const int rc = raise_smem(kern, smem, raised)) return rc;
   }
@@ -1230,13 +1261,12 @@ int few_launch(K kern, int smem, const AttnArgs& A, int64_t units, int S, int ro
   return BT_OK;
 }
 
-template <int W>
+template <int DP, int W>
 int few_run(const AttnArgs& A, bool half, int64_t units, int S, int row_tiles) {
-  if (half)
-    return A.D <= 64 ? few_launch<W>(attn_few_kernel<64, W>, FewShape<64, kFewRows, W>::kSmem, A, units, S, row_tiles)
-                     : few_launch<W>(attn_few_kernel<128, W>, FewShape<128, kFewRows, W>::kSmem, A, units, S, row_tiles);
-  return A.D <= 64 ? few_launch<W>(attn_few32_kernel<64, W>, FewShape<64, kFewRows32, W>::kSmem, A, units, S, row_tiles)
-                   : few_launch<W>(attn_few32_kernel<128, W>, FewShape<128, kFewRows32, W>::kSmem, A, units, S, row_tiles);
+  using F16 = FewShape<DP, kFewRows, W>;
+  static_assert(F16::kSmem <= F16::kRing, "the parts lie over the ring");
+  if (half) return few_launch<W, attn_few_kernel<DP, W>>(F16::kRing, A, units, S, row_tiles);
+  return few_launch<W, attn_few32_kernel<DP, W>>(FewShape<DP, kFewRows32, W>::kSmem, A, units, S, row_tiles);
 }
 
 // A tensor map over [B, H, T, D] (innermost D), 64 x 128 boxes; false where
@@ -1372,8 +1402,10 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
     int S = 1;
     while (S < 8 && units * S < 3 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * 4 * 64) S *= 2;
     if (units * S < INT32_MAX)
-      return S == 8 && units * S < di.sm_count ? few_run<8>(A, half, units, S, (int)row_tiles)
-                                               : few_run<4>(A, half, units, S, (int)row_tiles);
+      return D <= 64 ? (S == 8 && units * S < di.sm_count ? few_run<64, 8>(A, half, units, S, (int)row_tiles)
+                                                          : few_run<64, 4>(A, half, units, S, (int)row_tiles))
+                     : (S == 8 && units * S < di.sm_count ? few_run<128, 8>(A, half, units, S, (int)row_tiles)
+                                                          : few_run<128, 4>(A, half, units, S, (int)row_tiles));
   }
   if (!half && A.Tk > 0) {
     const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = A.B * A.H * q_tiles;
