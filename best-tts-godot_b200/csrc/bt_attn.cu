@@ -645,8 +645,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // ---- few queries ---------------------------------------------------------------
 // A step of generation: the queries that share a key head (Tq of each of its
 // G query heads) are rows of one or a few 16-row tiles, and the time is that
-// of reading K and V once.  A warp takes 16 keys at a time, fetched three
-// steps deep into a ring of its own (cp.async), as operands of 16 x 8 x 16
+// of reading K and V once.  A warp takes 16 keys at a time, fetched a step or
+// two ahead into a ring of its own (cp.async), as operands of 16 x 8 x 16
 // products (far below the tensor cores' rate here):
 //   S = Q K^T  the order of the summed dims is free, so a lane's 16 bytes of a
 //              key row are dims 8c..8c+7 of two products, Q permuted alike;
@@ -674,8 +674,10 @@ struct FewShape {
   static constexpr int kPart = ROWS * kPitch;                 // floats
   static constexpr int kSmem = W * kPart * 4;
   // the float16 form's ring: 16 rows of K, then of V, for each step; the parts
-  // lie over it at the end
-  static constexpr int kSteps = 3, kRow = DP * 2, kStep = 2 * 16 * kRow;
+  // lie over it at the end.  32 x 16 heads, one query, 2000 keys of 64: 46 us
+  // with two steps (5.7 TB/s), 52 with three, 62 with four; 8 x 8 key heads,
+  // 8192 keys of 128: 72 us with two, 62 with three
+  static constexpr int kSteps = DP == 64 ? 2 : 3, kRow = DP * 2, kStep = 2 * 16 * kRow;
   static constexpr int kRing = W * kSteps * kStep;
 };
 
@@ -1398,7 +1400,8 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   if (A.Tk > 0 && pieces && (row_tiles == 1 || few_us < tile_us)) {
     // the keys split over a cluster, then over more warps, until the GPU is
     // full or a warp is down to four steps of 16 keys (32 x 16 heads, one
-    // query over 2000 keys: 54 us in 512 CTAs, 61 in 1024, 74 in 2048)
+    // query over 2000 keys, before the ring: 54 us in 512 CTAs, 61 in 1024, 74
+    // in 2048)
     int S = 1;
     while (S < 8 && units * S < 3 * (int64_t)di.sm_count && A.Tk >= (int64_t)2 * S * 4 * 64) S *= 2;
     if (units * S < INT32_MAX)
