@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 #include "bt_ops.h"
 #include "bt_internal.h"
 #include "bt_pk.h"
@@ -1127,22 +1128,28 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       const int key = k0 + kg + 16 * j;
       in[j] = key < n && (!mask || mask[key * A.mask_sk]);
     }
+    const int left = n - k0 < kKeys32 ? n - k0 : kKeys32;
     float2 s2[8][4] = {};
+    auto score = [&](auto groups) {   // of every sixteen keys, the first `groups`
+      constexpr int kGroups = decltype(groups)::value;
 #pragma unroll(DP == 64 ? 2 : 1)
-    for (int d = 0; d < D; d += 4) {
-      float4 kk[4];
+      for (int d = 0; d < D; d += 4) {
+        float4 kk[kGroups];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kk[j] = *reinterpret_cast<const float4*>(ks + (kg + 16 * j) * Sh::kD + d);
+        for (int j = 0; j < kGroups; ++j) kk[j] = *reinterpret_cast<const float4*>(ks + (kg + 16 * j) * Sh::kD + d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 qq = *reinterpret_cast<const float4*>(qs + (rg + 16 * i) * Sh::kD + d);
+        for (int i = 0; i < 8; ++i) {
+          const float4 qq = *reinterpret_cast<const float4*>(qs + (rg + 16 * i) * Sh::kD + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s2[i][j] = pk_fma(make_float2(qq.x, qq.y), make_float2(kk[j].x, kk[j].y), s2[i][j]);
-          s2[i][j] = pk_fma(make_float2(qq.z, qq.w), make_float2(kk[j].z, kk[j].w), s2[i][j]);
+          for (int j = 0; j < kGroups; ++j) {
+            s2[i][j] = pk_fma(make_float2(qq.x, qq.y), make_float2(kk[j].x, kk[j].y), s2[i][j]);
+            s2[i][j] = pk_fma(make_float2(qq.z, qq.w), make_float2(kk[j].z, kk[j].w), s2[i][j]);
+          }
         }
       }
-    }
+    };
+    if (left > 16) score(std::integral_constant<int, 4>());
+    else score(std::integral_constant<int, 1>());
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float s[4], mn = m[i];
@@ -1170,7 +1177,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
     }
     __syncwarp();
 #pragma unroll 2
-    for (int k = 0; k < kKeys32; k += 2) {
+    for (int k = 0; k < left; k += 2) {   // (weights past the last key are 0, value rows zeros)
       float4 v0[J], v1[J];
 #pragma unroll
       for (int j = 0; j < J; ++j) {
@@ -1386,17 +1393,19 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   const bool pieces = rows16(A.q, A.qs, A.B, A.H, A.Tq, D, per) && rows16(A.k, A.ks, A.B, Hk, A.Tk, D, per) &&
                       rows16(A.v, A.vs, A.B, Hk, A.Tk, D, per);
   // The form with the least estimated time (us; measured with 1 to 64 batch
-  // entries, 1 to 16 heads, 32 to 1024 queries over 100 to 4096 keys): rows
-  // straight from global memory pay for every tile of rows and step of keys;
-  // the tiled forms for every round of CTAs and tile of keys.
+  // entries, 1 to 16 heads, 1 to 4000 queries over 6 to 4096 keys): rows
+  // straight from global memory pay for every tile of rows (a CTA's start and
+  // join) and step of 16 keys; the tiled forms for every round of CTAs and its
+  // tiles of keys.
   //   float16, 1 x 1 head,   256 queries, 4096 keys of 64: 21 against 54 us
   //            4 x 8 heads,  256 queries, 1000 keys of 64: 46 against 20 us
-  const double waves = ceil((double)(A.B * A.H * ((A.Tq + (half ? 2 * kTile : kRows32) - 1) / (half ? 2 * kTile : kRows32))) /
-                            di.sm_count);
-  const double few_us = half ? 17 + (double)units * (A.Tk / 16 + 1) * (D <= 64 ? 1.0e-3 : 3.0e-3)
-                             : 17 + (double)units * (A.Tk / 16 + 1) * (D <= 64 ? 1.6e-3 : 3.2e-3);
-  const double tile_us = half ? 9 + waves * (A.Tk / kTile + 1) * (D <= 64 ? 1.4 : 1.8)
-                              : 9 + waves * (A.Tk / kKeys32 + 1) * (D <= 64 ? 8.0 : 16.0);
+  //   float32, 2 x 4 heads,  256 queries, 1000 keys of 64: 61 against 135 us
+  //            4 x 32 heads, 4249 queries, 6 keys of 32: 1540 against 180 us
+  const int q_rows = half ? 2 * kTile : kRows32, k_rows = half ? kTile : kKeys32;
+  const double waves = ceil((double)(A.B * A.H * ((A.Tq + q_rows - 1) / q_rows)) / di.sm_count);
+  const double steps = (double)(A.Tk / 16 + 1), tiles = (double)((A.Tk + k_rows - 1) / k_rows);
+  const double few_us = 17 + (double)units * (10e-3 + steps * (half ? (D <= 64 ? 0.7e-3 : 2.5e-3) : (D <= 64 ? 1.0e-3 : 3.5e-3)));
+  const double tile_us = 9 + waves * (half ? 2.5 + tiles * (D <= 64 ? 1.5 : 1.9) : 3 + tiles * (D <= 64 ? 8.8 : 16.5));
   if (A.Tk > 0 && pieces && (row_tiles == 1 || few_us < tile_us)) {
     // the keys split over a cluster, then over more warps, until the GPU is
     // full or a warp is down to four steps of 16 keys (32 x 16 heads, one
