@@ -1072,7 +1072,7 @@ __device__ __forceinline__ void cp_async_or_zero(unsigned dst, const float* src,
 }
 
 template <int DP, int N>   // N: values a copy (4 where every row is 16-byte pieces)
-__global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_constant__ AttnArgs A, int q_tiles) {
+__global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_constant__ AttnArgs A, int q_tiles, int S) {
   using Sh = Shape32<DP>;
   constexpr int J = DP / 64;
   extern __shared__ __align__(16) float sm32[];
@@ -1080,8 +1080,9 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
   float* ps = qs + Sh::kQ;
   float* kv = ps + Sh::kPt;
   const int tid = threadIdx.x, lane = tid & 31, kg = lane & 15, rg = tid >> 4;
-  const uint32_t u = blockIdx.x / (unsigned)q_tiles;
-  const int64_t t0 = (int64_t)(blockIdx.x % (unsigned)q_tiles) * kRows32;
+  const unsigned rank = S > 1 ? cluster_rank() : 0;
+  const uint32_t cta = blockIdx.x / (unsigned)S, u = cta / (unsigned)q_tiles;
+  const int64_t t0 = (int64_t)(cta % (unsigned)q_tiles) * kRows32;
   const int64_t b = u / (uint32_t)A.H, h = u - b * A.H, hk = h / A.G;
   const int n = (int)keys_of(A, b), D = A.D;
   const uint8_t* mask = A.mask ? A.mask + b * A.mask_sb : nullptr;
@@ -1115,13 +1116,16 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
   float m[8], l[8] = {};
 #pragma unroll
   for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
-  if (n > 0) fetch(0, 0);
-  for (int k0 = 0, buf = 0; k0 < n; k0 += kKeys32) {
+  // this CTA's keys: whole tiles
+  const int key_tiles = (n + kKeys32 - 1) / kKeys32;
+  const int first = (int)((int64_t)key_tiles * rank / S) * kKeys32, end = (int)((int64_t)key_tiles * (rank + 1) / S) * kKeys32;
+  if (first < end) fetch(first, 0);
+  for (int k0 = first, buf = 0; k0 < end; k0 += kKeys32) {
     const float* ks = kv + buf * 2 * Sh::kKt;
     const float* vs = ks + Sh::kKt;
     asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     __syncthreads();   // this tile is there, and the last one is read by nobody any more
-    if (Sh::kBufs == 2 && k0 + kKeys32 < n) fetch(k0 + kKeys32, buf ^ 1);
+    if (Sh::kBufs == 2 && k0 + kKeys32 < end) fetch(k0 + kKeys32, buf ^ 1);
     bool in[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1200,14 +1204,31 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       buf ^= 1;
     } else {
       __syncthreads();
-      if (k0 + kKeys32 < n) fetch(k0 + kKeys32, 0);
+      if (k0 + kKeys32 < end) fetch(k0 + kKeys32, 0);
     }
+  }
+  if (S > 1) {
+    // the cluster's parts -- O, then a row's maximum and sum behind it, where Q
+    // was -- are joined by the CTA that owns the row (r mod S), in a fixed order
+    asm volatile("cp.async.wait_all;\n" ::: "memory");   // (a CTA without keys still has Q on its way)
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = rg + 16 * i;
 #pragma unroll
     for (int z = 1; z < 16; z *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], z);
+    if (S > 1) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        *reinterpret_cast<float4*>(qs + r * Sh::kD + 4 * kg + 64 * j) =
+            make_float4(o[i][2 * j].x, o[i][2 * j].y, o[i][2 * j + 1].x, o[i][2 * j + 1].y);
+      if (kg == 0) {
+        qs[r * Sh::kD + DP] = m[i];
+        qs[r * Sh::kD + DP + 1] = l[i];
+      }
+      continue;
+    }
     if (r >= rows) continue;
     float* out = (float*)A.out + b * A.os[0] + h * A.os[1] + (t0 + r) * A.os[2];
 #pragma unroll
@@ -1217,15 +1238,60 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       if (d < D) out[d * A.os[3]] = m[i] == -INFINITY ? 0.0f : __fdiv_rn(num, l[i]);
     }
   }
+  if (S > 1) {
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const unsigned part = smem_u32(qs);
+    auto at = [&](int k, int r, int col) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];\n"
+                   : "=f"(v)
+                   : "r"(cluster_addr(part + (unsigned)(r * Sh::kD + col) * 4, k))
+                   : "memory");
+      return v;
+    };
+    for (int i = tid; i < kRows32 / S * DP; i += kThreads32) {
+      const int r = i / DP * S + (int)rank, d = i % DP;
+      if (r >= rows || d >= D) continue;
+      float mx = -INFINITY, num = 0.0f, den = 0.0f;
+      for (int k = 0; k < S; ++k) mx = max3(mx, at(k, r, DP), -INFINITY);
+      if (mx != -INFINITY)
+        for (int k = 0; k < S; ++k) {
+          const float pm = at(k, r, DP), f = pm == -INFINITY ? 0.0f : ex2((pm - mx) * cs);
+          num = fmaf(at(k, r, d), f, num);
+          den = fmaf(at(k, r, DP + 1), f, den);
+        }
+      ((float*)A.out)[b * A.os[0] + h * A.os[1] + (t0 + r) * A.os[2] + d * A.os[3]] =
+          mx == -INFINITY ? 0.0f : __fdiv_rn(num, den);
+    }
+    __syncwarp();   // no CTA of the cluster leaves while its shared memory is read
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 template <int DP, int N>
-int attn_f32_launch(const AttnArgs& A, int64_t ctas, int q_tiles) {
+int attn_f32_launch(const AttnArgs& A, int64_t ctas, int q_tiles, int S) {
   auto kern = attn_f32_kernel<DP, N>;
   static bool raised[64];
   if (const int rc = raise_smem(kern, Shape32<DP>::kSmem, raised)) return rc;
-  kern<<<(unsigned)ctas, kThreads32, Shape32<DP>::kSmem, cur_stream()>>>(A, q_tiles);
-  return check_launch("bt_attention");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas * S));
+  cfg.blockDim = dim3(kThreads32);
+  cfg.dynamicSmemBytes = Shape32<DP>::kSmem;
+  cfg.stream = cur_stream();
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)S, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, A, q_tiles, S);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(BT_ECUDA, "bt_attention: launch failed: %s", cudaGetErrorString(e));
+  }
+  return BT_OK;
 }
 
 // Rows of 16-byte pieces (`per` values each) that the loads above can take.
@@ -1405,7 +1471,12 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   const double waves = ceil((double)(A.B * A.H * ((A.Tq + q_rows - 1) / q_rows)) / di.sm_count);
   const double steps = (double)(A.Tk / 16 + 1), tiles = (double)((A.Tk + k_rows - 1) / k_rows);
   const double few_us = 17 + (double)units * (10e-3 + steps * (half ? (D <= 64 ? 0.7e-3 : 2.5e-3) : (D <= 64 ? 1.0e-3 : 3.5e-3)));
-  const double tile_us = 9 + waves * (half ? 2.5 + tiles * (D <= 64 ? 1.5 : 1.9) : 3 + tiles * (D <= 64 ? 8.8 : 16.5));
+  // (float32 tiles: the keys split over a cluster while that still fits one round)
+  const int64_t ctas32 = A.B * A.H * ((A.Tq + kRows32 - 1) / kRows32);
+  int split32 = 1;
+  while (split32 < 8 && ctas32 * split32 * 2 <= di.sm_count && tiles >= 4 * split32) split32 *= 2;
+  const double tile_us =
+      9 + waves * (half ? 2.5 + tiles * (D <= 64 ? 1.5 : 1.9) : 3 + 2 * (split32 > 1) + tiles / split32 * (D <= 64 ? 8.8 : 16.5));
   if (A.Tk > 0 && pieces && (row_tiles == 1 || few_us < tile_us)) {
     // the keys split over a cluster, then over more warps, until the GPU is
     // full or a warp is down to four steps of 16 keys (32 x 16 heads, one
@@ -1420,11 +1491,11 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
                                                           : few_run<128, 4>(A, half, units, S, (int)row_tiles));
   }
   if (!half && A.Tk > 0) {
-    const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = A.B * A.H * q_tiles;
+    const int64_t q_tiles = (A.Tq + kRows32 - 1) / kRows32, ctas = ctas32;
     if (ctas < INT32_MAX && pieces)
-      return D <= 64 ? attn_f32_launch<64, 4>(A, ctas, (int)q_tiles) : attn_f32_launch<128, 4>(A, ctas, (int)q_tiles);
+      return D <= 64 ? attn_f32_launch<64, 4>(A, ctas, (int)q_tiles, split32) : attn_f32_launch<128, 4>(A, ctas, (int)q_tiles, split32);
     if (ctas < INT32_MAX)
-      return D <= 64 ? attn_f32_launch<64, 1>(A, ctas, (int)q_tiles) : attn_f32_launch<128, 1>(A, ctas, (int)q_tiles);
+      return D <= 64 ? attn_f32_launch<64, 1>(A, ctas, (int)q_tiles, split32) : attn_f32_launch<128, 1>(A, ctas, (int)q_tiles, split32);
   }
   if (half && A.Tk > 0) {
     AttnTc P{};

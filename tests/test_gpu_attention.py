@@ -72,6 +72,32 @@ def test_many_items(gpu_runtime, B, H, Tq, Tk, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D", [64, 128, 36])
+def test_few_tiles_over_long_keys(gpu_runtime, D, dtype):
+    """Fewer tiles of queries than SMs, so that the keys are split: lengths that
+    leave whole parts without keys, and NaN in one part."""
+    rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(D)
+    B, H, Tq, Tk = 4, 2, 900, 2500
+    q, k, v = (_states(g, B, H, t, D, dtype, "token") for t in (Tq, Tk, Tk))
+    lengths = torch.tensor([0, 1, 70, Tk], dtype=torch.int32, device="cuda")
+    _run(rt, q, k, v, "all")
+    o = _run(rt, q, k, v, "lengths", lengths=lengths)
+    assert (o[0] == 0).all()
+    mask = torch.zeros(B, Tk, dtype=torch.bool, device="cuda")
+    mask[1, 2400:] = True
+    mask[2, 1200] = True
+    mask[3, ::3] = True
+    o = _run(rt, q, k, v, "mask", key_mask=mask)
+    k2 = k.clone()
+    k2[3, 1, 2490, 0] = float("nan")
+    full = rt.attention(q, k, v)
+    bad = rt.attention(q, k2, v)
+    assert bad[3, 1].isnan().all()
+    bad[3, 1] = full[3, 1]
+    assert torch.equal(bad, full)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 @pytest.mark.parametrize("D", [64, 128])
 def test_many_items_growing_and_non_finite(gpu_runtime, D, dtype):
     """Rows whose reference moves in every key tile, beside rows where it never
