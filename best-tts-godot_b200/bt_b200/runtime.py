@@ -916,7 +916,10 @@ class BtRuntime:
         rows = math.prod(lead)
         fits = _row_pitch_ok(a) and _row_pitch_ok(w) and a_scale.is_contiguous()
         dt = TORCH_TO_NP[out_dtype]
-        return (tensor_desc(a), make_tensor(0, np.float32, (rows,)), tensor_desc(w), tensor_desc(w_scale),
+        # (operands without values may have any strides)
+        ad = tensor_desc(a) if a.numel() else make_tensor(0, np.int8, (rows, K))
+        wd = tensor_desc(w) if w.numel() else make_tensor(0, np.int8, (N, K))
+        return (ad, make_tensor(0, np.float32, (rows,)), wd, tensor_desc(w_scale),
                 None if bias is None else tensor_desc(bias), make_tensor(0, dt, (rows, N)), lead + (N,),
                 _c_strides(lead + (N,)), fits, rows * N)
 
@@ -1417,7 +1420,10 @@ def _axis_blocks(axes, shape):
 
 def _one_row_stride(t):
     """Whether t's leading axes collapse to one axis of constant stride over
-    rows of unit stride (rows of a C-contiguous tensor, or of a wider buffer)."""
+    rows of unit stride (rows of a C-contiguous tensor, or of a wider buffer).
+    A tensor without values has nothing to stride over."""
+    if t.numel() == 0:
+        return True
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         return False
     n = 1
@@ -1441,7 +1447,9 @@ def _c_strides(shape):
 
 def _row_pitch_ok(t):
     """Rows of one stride, a multiple of 16 bytes above 0 (a broadcast row
-    has none)."""
+    has none); any where there are no values."""
+    if t.numel() == 0:
+        return True
     if not _one_row_stride(t):
         return False
     step = next((t.stride(d) for d in range(t.dim() - 2, -1, -1) if t.shape[d] != 1), 16)

@@ -181,6 +181,20 @@ def test_matmul_empty(gpu_runtime):
     assert torch.equal(rt.matmul_int8(a[:, :0], sa, w[:, :0], sw), torch.zeros(4, 8, device="cuda"))
 
 
+def test_matmul_and_quantize_empty_in_any_layout(gpu_runtime):
+    """Operands without values: allocated as such, or seen through odd strides."""
+    rt = gpu_runtime
+    a, w = torch.empty(4, 0, dtype=torch.int8, device="cuda"), torch.empty(8, 0, dtype=torch.int8, device="cuda")
+    sa, sw, b = torch.ones(4, device="cuda"), torch.ones(8, device="cuda"), torch.arange(8.0, device="cuda")
+    assert torch.equal(rt.matmul_int8(a, sa, w, sw, bias=b), b.expand(4, 8))
+    a3 = torch.empty(3, 2, 0, dtype=torch.int8, device="cuda").transpose(0, 1)
+    assert torch.equal(rt.matmul_int8(a3, torch.ones(2, 3, device="cuda"), w, sw, bias=b), b.expand(2, 3, 8))
+    none, rows = torch.empty(3, 0, 16, device="cuda"), torch.empty(3, 0, device="cuda")
+    assert rt.matmul_int8(none.char(), rows, torch.ones(8, 16, dtype=torch.int8, device="cuda"), sw).shape == (3, 0, 8)
+    q, s = rt.quantize_rows(none)
+    assert q.shape == (3, 0, 16) and s.shape == (3, 0)
+
+
 def test_matmul_refusals(gpu_runtime):
     rt = gpu_runtime
     a, sa, w, sw, b = _case(7, 4, 8, 32, True)

@@ -98,3 +98,12 @@ def test_empty_results_need_no_gpu(lib):
     assert lib.bt_matmul_int8(_ref(a), _ref(sa), _ref(w), _ref(sw), None, _ref(o)) == 0
     q, k, o = T(F16, 2, 4, 0, 64), T(F16, 2, 2, 7, 64), T(F16, 2, 4, 0, 64)
     assert lib.bt_attention(_ref(q), _ref(k), _ref(k), None, None, 0.125, _ref(o)) == 0
+
+
+@pytest.mark.parametrize("shape", [(4, 0), (2, 3, 0), (3, 0, 16), (0, 5)])
+def test_operands_without_values_need_no_copy(shape):
+    torch = pytest.importorskip("torch")
+    from bt_b200.runtime import _one_row_stride, _row_pitch_ok
+    for t in (torch.empty(shape, dtype=torch.int8), torch.empty(shape[::-1], dtype=torch.int8).permute(
+            *reversed(range(len(shape))))):
+        assert _one_row_stride(t) and _row_pitch_ok(t)
