@@ -944,6 +944,8 @@ class BtRuntime:
         are read in place (a [B, T, H, D] projection permuted to
         [B, H, T, D])."""
         plans = self._plans("attention")
+        if scale is not None:
+            scale = float(scale)   # by value: a tensor as a key would be its identity
         try:
             key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape,
                    v.stride(), v.dtype, v.get_device(), scale,
@@ -985,7 +987,7 @@ class BtRuntime:
         Hk, Tk = int(k.shape[1]), int(k.shape[2])
         if k.shape[0] != B or k.shape[3] != D or (H % Hk if Hk else H):
             raise ValueError(f"{what}: q of shape {tuple(q.shape)} cannot attend to k of shape {tuple(k.shape)}")
-        scale = 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale)
+        scale = 1.0 / math.sqrt(max(D, 1)) if scale is None else scale
         if lengths is not None:
             if lengths.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"{what}: lengths must be int32 or int64, not {lengths.dtype}")

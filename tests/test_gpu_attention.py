@@ -193,6 +193,16 @@ def test_scale(gpu_runtime, scale):
             _run(gpu_runtime, q, k, v, f"{scale}", scale=scale)
 
 
+def test_scale_is_taken_by_value(gpu_runtime):
+    """One scalar tensor whose value changes between two calls."""
+    g = torch.Generator("cuda").manual_seed(12)
+    q, k, v = (_states(g, 1, 2, t, 64, F32) for t in (3, 50, 50))
+    s = torch.tensor(0.1)
+    for x in (0.1, 0.7):
+        s.fill_(x)
+        assert torch.equal(gpu_runtime.attention(q, k, v, scale=s), gpu_runtime.attention(q, k, v, scale=float(s)))
+
+
 def test_non_finite_values_stay_in_their_rows(gpu_runtime):
     g = torch.Generator("cuda").manual_seed(2)
     for dtype in (F16, F32):
