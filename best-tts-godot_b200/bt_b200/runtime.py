@@ -942,7 +942,8 @@ class BtRuntime:
         part; keys that do not are never looked at, and a row without any
         gives zeros.  scale defaults to 1 / sqrt(D).  Views of any strides
         are read in place (a [B, T, H, D] projection permuted to
-        [B, H, T, D])."""
+        [B, H, T, D]), except that long float16 ones whose rows do not start
+        on 16-byte boundaries are copied to such rows first."""
         plans = self._plans("attention")
         if scale is not None:
             scale = float(scale)   # by value: a tensor as a key would be its identity
@@ -962,12 +963,15 @@ class BtRuntime:
             if key_mask is not None:
                 self._check_here("attention", key_mask=key_mask)
             plan = self._keep_plan(plans, key, self._attention_plan(q, k, v, lengths, key_mask, scale))
-        qd, kd, vd, ld, md, od, sc, shape, strides, numel = plan
+        qd, kd, vd, ld, md, od, sc, shape, strides, numel, pieces = plan
         out = torch.empty_strided(shape, strides, dtype=q.dtype, device=self.device)
         if numel:
-            qd.data = q.data_ptr()
-            kd.data = k.data_ptr()
-            vd.data = v.data_ptr()
+            pq, pk, pv = q.data_ptr(), k.data_ptr(), v.data_ptr()
+            if pieces is not None and not (pieces and (pq | pk | pv) & 15 == 0):
+                rows = [self._half_rows(t) for t in (q, k, v)]   # (kept until the launch)
+                qd, kd, vd = (tensor_desc(t) for t in rows)
+            else:
+                qd.data, kd.data, vd.data = pq, pk, pv
             od.data = out.data_ptr()
             if lengths is not None:
                 ld.data = lengths.data_ptr()
@@ -1004,8 +1008,32 @@ class BtRuntime:
             strides[ax] = acc
             acc *= shape[ax]
         od = make_tensor(0, np_dtype(q), shape, strides)
+        # float16 rows that are no 16-byte pieces take the kernel for any
+        # strides (a key after the other, every row's keys from global memory),
+        # or copies in such rows the others.  By estimates in us; measured,
+        # copied / as they are:
+        #   1 x 1 heads,    1 query,     10 keys of 36:   69 /   14
+        #   32 x 16 heads,  1 query,   2000 keys of 36: 1658 /  933
+        #   1 x 8 heads,    1 query,    500 keys of 36:   86 /  134
+        #   8 x 12 heads, 300 queries,  300 keys of 36:  172 /  767
+        #   the same of 64, one value off 16 bytes:       80 / 2307
+        #   4 x 8 heads, 1000 queries, 1000 keys of 100: 208 / 5255
+        pieces = None   # (any rows will do)
+        if q.dtype == torch.float16:
+            copies = 65 + (q.numel() + k.numel() + v.numel()) * (20e-6 if D % 8 else 6e-6)
+            if Tk * (0.4 + B * H * int(q.shape[2]) * 0.1e-3) > copies:
+                pieces = _half_pieces(q) and _half_pieces(k) and _half_pieces(v)
         return (tensor_desc(q), tensor_desc(k), tensor_desc(v), None if lengths is None else tensor_desc(lengths),
-                None if key_mask is None else tensor_desc(key_mask), od, scale, shape, tuple(strides), math.prod(shape))
+                None if key_mask is None else tensor_desc(key_mask), od, scale, shape, tuple(strides), math.prod(shape),
+                pieces)
+
+    def _half_rows(self, t):
+        """t itself where its rows are 16-byte pieces, else a copy in such rows."""
+        if _half_pieces(t) and t.data_ptr() & 15 == 0:
+            return t
+        D = int(t.shape[-1])
+        buf = torch.empty(tuple(t.shape[:-1]) + ((D + 7) // 8 * 8,), dtype=t.dtype, device=self.device)
+        return self._copy_desc(tensor_desc(t), np_dtype(t), buf[..., :D])
 
     def _as_f32(self, t):
         dt = np_dtype(t)
@@ -1437,6 +1465,14 @@ def _one_row_stride(t):
                 return False
             n *= int(t.shape[d])
     return True
+
+
+def _half_pieces(t):
+    """Whether the rows of a float16 [B, H, T, D] lie at multiples of 16 bytes
+    from its start (one row for all T does not)."""
+    if t.shape[3] > 1 and t.stride(3) != 1 or t.shape[2] > 1 and t.stride(2) == 0:
+        return False
+    return all(t.shape[d] == 1 or t.stride(d) % 8 == 0 for d in range(3))
 
 
 def _c_strides(shape):

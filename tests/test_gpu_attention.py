@@ -193,6 +193,53 @@ def test_scale(gpu_runtime, scale):
             _run(gpu_runtime, q, k, v, f"{scale}", scale=scale)
 
 
+@pytest.mark.parametrize("Hk", [4, 1])
+def test_half_rows_off_16_bytes(gpu_runtime, Hk):
+    """Views that are copied to aligned rows first: the aligned call's bits,
+    in q's axis order; a row that stands for all keys; a captured call."""
+    rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(13)
+    n = torch.tensor([400, 33], dtype=torch.int32, device="cuda")
+    for Tq, D in ((1, 64), (300, 64), (300, 128)):
+        q, k, v = _states(g, 2, 4, Tq, D, F16, "token"), _states(g, 2, Hk, 400, D, F16), _states(g, 2, Hk, 400, D, F16)
+        want = rt.attention(q, k, v, lengths=n)
+
+        def off(t):
+            room = torch.full(tuple(t.shape[:-1]) + (D + 3,), float("nan"), dtype=F16, device="cuda")
+            room[..., 1:D + 1].copy_(t)
+            return room[..., 1:D + 1]
+        for args in ((off(q), k, v), (q, off(k), v), (q, k, off(v)), (off(q), off(k), off(v))):
+            assert torch.equal(rt.attention(*args, lengths=n), want)
+        p = torch.empty(2 * Tq * 4 * D + 1, dtype=F16, device="cuda")[1:].view(2, Tq, 4, D).permute(0, 2, 1, 3)
+        p.copy_(q)
+        o = rt.attention(p, k, v, lengths=n)
+        assert torch.equal(o, want) and o.stride() == want.stride()
+        same = k[:, :, 7:8].expand(2, Hk, 400, D)
+        assert torch.equal(rt.attention(q, same, v, lengths=n), rt.attention(q, same.contiguous(), v, lengths=n))
+        args, s = (off(q), off(k), off(v)), torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            rt.attention(*args, lengths=n)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            o = rt.attention(*args, lengths=n)
+        args[0].neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, rt.attention(-q, k, v, lengths=n))
+
+
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,D", [(2, 4, 2, 300, 300, 36), (1, 2, 1, 150, 700, 7), (2, 2, 2, 260, 500, 100),
+                                            (1, 2, 2, 1, 900, 1), (1, 3, 3, 140, 400, 65)])
+def test_half_dims_off_16_bytes(gpu_runtime, B, H, Hk, Tq, Tk, D):
+    g = torch.Generator("cuda").manual_seed(14)
+    mask = torch.rand(B, Tk, generator=g, device="cuda") < 0.7
+    mask[-1] = False
+    for layout in ("head", "token"):
+        q, k, v = (_states(g, B, h, t, D, F16, layout) for h, t in ((H, Tq), (Hk, Tk), (Hk, Tk)))
+        _run(gpu_runtime, q, k, v, layout)
+        _run(gpu_runtime, q, k, v, layout, key_mask=mask)
+
+
 def test_scale_is_taken_by_value(gpu_runtime):
     """One scalar tensor whose value changes between two calls."""
     g = torch.Generator("cuda").manual_seed(12)
