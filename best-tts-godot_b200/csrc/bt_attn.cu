@@ -1051,7 +1051,7 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
 // rows of keys that take no part are filled with zeros), for dims up to 64
 // the next tile while this one is worked on.  Bound by the FMA pipe.
 // Measured: 37 TFLOP/s at 8 x 16 heads of 1024 x 1024 x 64, half of the FMA
-// pipe's rate, and 168 us at 8 x 12 heads of up to 510 x 510 x 64 (three rounds
+// pipe's rate, and 172 us at 8 x 12 heads of up to 510 x 510 x 64 (three rounds
 // of CTAs); 8 x 8 sums a thread with two CTAs of 128 threads on an SM came to
 // the same (36 TFLOP/s, 175 us).
 constexpr int kRows32 = 128, kKeys32 = 64, kThreads32 = 256;

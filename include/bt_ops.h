@@ -350,7 +350,8 @@ int bt_quantize_rows(const bt_tensor* x, const bt_tensor* q,
  * float16 [..., N].  The sum is an exact int32; it is converted to float32,
  * scaled, biased, and rounded to float16 once where out is float16.  K at
  * most 131071 (beyond it the sum could overflow: BT_ETOOBIG); K = 0 gives
- * the bias, or 0.
+ * the bias, or 0.  The rows of a and w start on 16-byte boundaries, each row
+ * a place of its own (BT_EUNSUPPORTED otherwise).
  * No counterpart in the reference, whose MatMulInteger nodes have one
  * activation scale for the whole tensor. */
 int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
@@ -362,8 +363,8 @@ int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
  * values k, v [B, Hk, Tk, D] of another length (an encoder's states, or the
  * queries' own sequence); query head h reads key head h / (H / Hk), so H is a
  * multiple of Hk.  One dtype for q, k, v and out: float32 or float16; any
- * strides (a permuted [B, T, H, D] projection is read in place); D at most
- * 128.  lengths (NULL: Tk): int32 or int64 [B], the keys of each batch entry,
+ * strides (a permuted [B, T, H, D] projection is read in place; float16 rows
+ * off 16-byte boundaries take a slow kernel); D at most 128.  lengths (NULL: Tk): int32 or int64 [B], the keys of each batch entry,
  * clamped to 0..Tk.  key_mask (NULL: none): bool [B, Tk], true where a key
  * takes part.  Keys that do not take part are never looked at, whatever their
  * k and v rows hold; a query row no key takes part in gives zeros.  scale:
