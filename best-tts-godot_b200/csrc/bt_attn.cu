@@ -852,9 +852,11 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
       float top = max3(max3(s[0][2 * h], s[0][2 * h + 1], s[1][2 * h]), s[1][2 * h + 1], m[h]);
       top = max3(top, __shfl_xor_sync(0xffffffffu, top, 1), -INFINITY);
       const float mn = max3(top, __shfl_xor_sync(0xffffffffu, top, 2), -INFINITY);
-      const float base = mn == -INFINITY ? 0.0f : mn * cs;
+      // (the reference is subtracted before the scaling: as a scaled and rounded
+      // product of a large score it would lift a weight past float16's range)
+      const float base = mn == -INFINITY ? 0.0f : mn;
       if (__any_sync(0xffffffffu, !(mn <= m[h]))) {
-        const float keep = ex2(m[h] * cs - base);   // (m = -inf: 0)
+        const float keep = ex2((m[h] - base) * cs);   // (m = -inf: 0)
         m[h] = mn;
         l[h] *= keep;
 #pragma unroll
@@ -866,7 +868,7 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[e] = ex2(fmaf(s[e >> 1][2 * h + (e & 1)], cs, -base));
+        p[e] = ex2((s[e >> 1][2 * h + (e & 1)] - base) * cs);
         l[h] += p[e];
       }
       // weights as float16, lifted by 2^7 off its subnormals (the sum is of
