@@ -152,12 +152,16 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // and the sum are rescaled) only when the maximum has grown by more than 2^8
 // in p: rescaling O costs a pass over tensor memory, and p <= 2^15 stays in
 // float16's range.  The 2^7 lifts small weights off float16's subnormals: a
-// weight loses precision only below 2^-21 of the reference.  P is rounded to
+// weight loses precision only below 2^-21 of the reference.  The exponent is
+// one fma of the score with 7 - m c, whose rounding is an error of up to 2^-14
+// while m c is below 2^11, and grows with it: to a factor past float16's range
+// at 2^24.  A row beyond 2^11 subtracts m from its scores first (a vote a key
+// tile and, in warps with such a row, a pass over the scores).  P is rounded to
 // float16 (the tensor cores' operand; relative error 2^-11 a weight, as a
 // float16 result has anyway); the row's sum is of the float32 weights.
 constexpr int kTile = 128;
 constexpr int kAttnThreads = 384;
-constexpr float kGrow = 8.0f, kLift = 7.0f;
+constexpr float kGrow = 8.0f, kLift = 7.0f, kFar = 2048.0f;
 
 struct AttnTc {
   AttnArgs a;
@@ -318,7 +322,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       if (pos.t0 + tile * kTile >= a.Tq) continue;
       const bool turns = pos.t0 + kTile < a.Tq;   // both tiles have work
       const uint8_t* mask = a.mask ? a.mask + pos.b * a.mask_sb : nullptr;
-      float m = -INFINITY, mc = 0.0f;   // the reference (-inf: no key yet) and m c - 7
+      float m = -INFINITY;          // the reference (-inf: no key yet)
+      float off = 0.0f, ref = 0.0f;   // p = 2^((s - ref) c + off)
       float2 l = {0.0f, 0.0f};
       uint8_t mb[4] = {1, 1, 1, 1};
       if (mask)
@@ -374,7 +379,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const float keep = grow ? (m == -INFINITY ? 0.0f : exp2f((m - top) * c)) : 1.0f;
           if (grow) {
             m = top;
-            mc = fmaf(top, c, -kLift);
+            off = fmaf(top, -c, kLift);
+            const bool far = fabsf(off) > kFar;
+            ref = far ? top : 0.0f;
+            off = far ? kLift : off;
             l.x *= keep;
             l.y *= keep;
           }
@@ -393,8 +401,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
             }
           }
         }
+        if (__any_sync(0xffffffffu, ref != 0.0f)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s[i][j] = __float_as_uint(__uint_as_float(s[i][j]) - ref);
+        }
         if (turns) my_turn();
-        const float2 c2 = {c, c}, mc2 = {-mc, -mc};
+        const float2 c2 = {c, c}, off2 = {off, off};
         float2 part_l[2] = {};
         // Pair x is scaled in step x, exponentiated in step x + 1, summed and
         // rounded in step x + 3, in this order (volatile): the special-function
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
         for (int x = 0; x < 64 + 3; ++x) {
           if (x < 64)
-            e[x] = pk_fma_v(make_float2(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, mc2);
+            e[x] = pk_fma_v(make_float2(__uint_as_float(s[x / 16][x % 16 * 2]), __uint_as_float(s[x / 16][x % 16 * 2 + 1])), c2, off2);
           if (x >= 1 && x <= 64) ex2_v(e[x - 1].x);
           if (x >= 3) part_l[x & 1] = pk_add(part_l[x & 1], e[x - 3]);
           if (x >= 1 && x <= 64) ex2_v(e[x - 1].y);
@@ -430,8 +444,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       // the result: O / l
       const float sum = l.x + l.y;
-      // (a row with a key has a weight of at least 2^-1)
-      const bool none = sum < 0x1p-60f;
+      const bool none = m == -INFINITY;
       const float inv = 1.0f / sum;
       __half* out = (__half*)a.out + pos.b * a.os[0] + pos.h * a.os[1] + t * a.os[2];
       if (n > 0) {
