@@ -86,12 +86,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
       if (in) {
         float dot = 0.0f;
         for (int d = 0; d < A.D; ++d) dot = __fmaf_rn(qsh[w][d], ldf(kp + j * A.ks[2] + d * A.ks[3]), dot);
-        s = dot * A.scale;
+        s = dot;   // (scaled as a difference to the maximum: the product alone may overflow)
       }
       float mx = s;
       for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.0f : mn;
-      const float keep = expf(m - base), p = in ? expf(s - base) : 0.0f;
+      const float keep = expf((m - base) * A.scale), p = in ? expf((s - base) * A.scale) : 0.0f;
       m = mn;
       float sum = p;
       for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);

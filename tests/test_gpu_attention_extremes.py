@@ -11,10 +11,10 @@ pytestmark = pytest.mark.gpu
 F16, F32 = torch.float16, torch.float32
 
 # (batch, heads, key heads, queries, keys, dim): few queries; tiles of queries, in
-# float32 with the keys split and not
+# float32 with the keys split and not; float16 rows that are read as they lie
 FORMS = [(2, 4, 2, 1, 700, 64), (2, 4, 2, 1, 700, 128), (2, 4, 2, 3, 100, 64), (2, 4, 2, 3, 100, 128), (2, 4, 2, 1, 700, 36),
          (4, 8, 4, 256, 700, 64), (4, 8, 4, 256, 700, 128), (4, 8, 4, 256, 700, 36), (8, 8, 4, 256, 300, 64), (8, 8,
-         4, 256, 300, 128), (8, 8, 4, 256, 300, 36)]
+         4, 256, 300, 128), (8, 8, 4, 256, 300, 36), (2, 4, 2, 3, 100, 36)]
 
 
 def attention_of_exact_scores(q, k, v, scale=None):
