@@ -368,7 +368,8 @@ int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
  * clamped to 0..Tk.  key_mask (NULL: none): bool [B, Tk], true where a key
  * takes part.  Keys that do not take part are never looked at, whatever their
  * k and v rows hold; a query row no key takes part in gives zeros.  scale:
- * positive and finite.  Scores, softmax and sums are float32.
+ * positive, at most 2^127 (BT_EINVAL otherwise).  Scores, softmax and sums are
+ * float32.
  * replaces: the MatMul, Mul, Add, Softmax, MatMul nodes of an attention block
  *           (ref_runtime.py:446-451, :269-273 + :599-600 for Mul, Add and
  *           Softmax), one dispatch each in the reference. */
