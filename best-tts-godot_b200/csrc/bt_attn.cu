@@ -9,6 +9,8 @@
 // and out = o / l, or 0 where no key takes part.  A key outside lengths or
 // the mask is never looked at: its score is replaced, not added to, and its
 // value row is left out, so NaN or infinities stored there have no effect.
+// Where every key that takes part scores -inf, l is 0 and the row 0 / 0: a
+// maximum of -inf does not mean that no key took part, so that is kept apart.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -77,11 +79,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
     __syncwarp();
     const int64_t n = keys_of(A, b);
     float m = -INFINITY, l = 0.0f, o[kMaxHeadDim / 32] = {};
+    bool any = false;   // a key took part
     for (int64_t j0 = 0; j0 < n; j0 += 32) {
       const int64_t j = j0 + lane;
       const bool in = j < n && (!A.mask || A.mask[b * A.mask_sb + j * A.mask_sk]);
       unsigned live = __ballot_sync(0xffffffffu, in);
       if (!live) continue;
+      any = true;
       float s = -INFINITY;
       if (in) {
         float dot = 0.0f;
@@ -112,7 +116,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 #pragma unroll
     for (int i = 0; i < kMaxHeadDim / 32; ++i)
       if (lane + 32 * i < A.D) {
-        const float y = l == 0.0f ? 0.0f : __fdiv_rn(o[i], l);
+        const float y = any ? __fdiv_rn(o[i], l) : 0.0f;
         if constexpr (sizeof(T) == 2) op[(lane + 32 * i) * A.os[3]] = __float2half_rn(y);
         else op[(lane + 32 * i) * A.os[3]] = y;
       }
@@ -325,6 +329,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       float m = -INFINITY;          // the reference (-inf: no key yet)
       float off = 0.0f, ref = 0.0f;   // p = 2^((s - ref) c + off)
       float2 l = {0.0f, 0.0f};
+      bool any = false;   // a key took part
       uint8_t mb[4] = {1, 1, 1, 1};
       if (mask)
 #pragma unroll
@@ -336,6 +341,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = __ballot_sync(0xffffffffu, mb[i] != 0);
           part = (w[0] & w[1] & w[2] & w[3]) != ~0u;
+          any |= (w[0] | w[1] | w[2] | w[3]) != 0;
           // the next tile's bytes, while this one is computed
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
       // the result: O / l
       const float sum = l.x + l.y;
-      const bool none = m == -INFINITY;
+      const bool none = mask ? !any : n == 0;
       const float inv = 1.0f / sum;
       __half* out = (__half*)a.out + pos.b * a.os[0] + pos.h * a.os[1] + t * a.os[2];
       if (n > 0) {
@@ -697,7 +703,8 @@ struct FewShape {
 
 // Joins the parts of all warps of the CTA, or of the cluster (each CTA then
 // takes the rows r = rank mod S), and stores the outputs.  The parts' O are
-// lifted by `lift` against their sums.
+// lifted by `lift` against their sums.  A part whose keys all scored -inf has
+// that maximum and a sum of NaN, one without keys a sum of 0.
 template <int DP, int ROWS, int W, typename T>
 __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, int rank, int64_t b, int64_t hk, int64_t row0,
                                          float cs, float lift) {
@@ -724,15 +731,18 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
     for (int k = 0; k < S; ++k)
       for (int w = 0; w < W; ++w) mx = max3(mx, at(k, w, DP), -INFINITY);
     float num = 0.0f, den = 0.0f;
-    if (mx != -INFINITY)
-      for (int k = 0; k < S; ++k)
-        for (int w = 0; w < W; ++w) {
-          const float pm = at(k, w, DP);
-          const float f = pm == -INFINITY ? 0.0f : exp2f((pm - mx) * cs);
-          num = fmaf(at(k, w, d), f, num);
-          den = fmaf(at(k, w, DP + 1), f, den);
+    for (int k = 0; k < S; ++k)
+      for (int w = 0; w < W; ++w) {
+        const float pm = at(k, w, DP);
+        if (pm == -INFINITY) {
+          if (mx == -INFINITY) den += at(k, w, DP + 1);
+          continue;
         }
-    const float y = mx == -INFINITY ? 0.0f : num / (den * lift);
+        const float f = exp2f((pm - mx) * cs);
+        num = fmaf(at(k, w, d), f, num);
+        den = fmaf(at(k, w, DP + 1), f, den);
+      }
+    const float y = mx == -INFINITY ? den : num / (den * lift);
     T* out = (T*)A.out + b * A.os[0] + (hk * A.G + gr / A.Tq) * A.os[1] + gr % A.Tq * A.os[2];
     if constexpr (sizeof(T) == 2) out[d * A.os[3]] = __float2half_rn(y);
     else out[d * A.os[3]] = y;
@@ -778,6 +788,7 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
   }
   float o[Sh::kO][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  bool any = false;   // a key took part
   const float cs = A.scale * 1.4426950408889634f;   // log2(e)
 
   // this CTA's keys: whole steps of 16, as even as they go
@@ -833,6 +844,7 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
         in[y] = key < n && (!mask || mask[key * A.mask_sk]);
       }
     }
+    any |= in[0] | in[1] | in[2] | in[3];
     float s[2][4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -903,10 +915,12 @@ __global__ void __launch_bounds__(32 * W) attn_few_kernel(const __grid_constant_
       }
     }
   }
+  any = __any_sync(0xffffffffu, any);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    if (any && m[h] == -INFINITY) l[h] = NAN;
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
   __syncthreads();   // every warp is done with its ring
@@ -954,6 +968,7 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
   };
   float4 q[R][Y], o[R][Y] = {};
   float m[R], l[R] = {};
+  bool any = false;   // a key took part
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int64_t gr = (int64_t)rt * R + r;
@@ -973,6 +988,7 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
     for (int t = 0; t < kAhead; ++t) {
       const int key = kStep * st + 4 * t + grp;
       in[t] = key < n && (!mask || mask[key * A.mask_sk]);
+      any |= in[t];
 #pragma unroll
       for (int y = 0; y < Y; ++y) {
         k[t][y] = ld4(kp + key * A.ks[2], y, key < n);
@@ -1022,6 +1038,7 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
   }
   // the four lane groups of the warp become one part
   float* mine = few_sm + warp * Sh::kPart;
+  any = __any_sync(0xffffffffu, any);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -1046,7 +1063,7 @@ __global__ void __launch_bounds__(32 * W) attn_few32_kernel(const __grid_constan
       for (int y = 0; y < Y; ++y) *reinterpret_cast<float4*>(mine + r * Sh::kPitch + 4 * (x + 8 * y)) = o[r][y];
       if (x == 0) {
         mine[r * Sh::kPitch + DP] = m[r];
-        mine[r * Sh::kPitch + DP + 1] = l[r];
+        mine[r * Sh::kPitch + DP + 1] = any && m[r] == -INFINITY ? NAN : l[r];
       }
     }
   }
@@ -1129,6 +1146,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
 
   float2 o[8][2 * J] = {};
   float m[8], l[8] = {};
+  bool any = false;   // a key took part
 #pragma unroll
   for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
   // this CTA's keys: whole tiles
@@ -1146,6 +1164,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
     for (int j = 0; j < 4; ++j) {
       const int key = k0 + kg + 16 * j;
       in[j] = key < n && (!mask || mask[key * A.mask_sk]);
+      any |= in[j];
     }
     const int left = n - k0 < kKeys32 ? n - k0 : kKeys32;
     float2 s2[8][4] = {};
@@ -1228,11 +1247,13 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
     asm volatile("cp.async.wait_all;\n" ::: "memory");   // (a CTA without keys still has Q on its way)
     __syncthreads();
   }
+  any = __any_sync(0xffffffffu, any);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = rg + 16 * i;
 #pragma unroll
     for (int z = 1; z < 16; z *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], z);
+    if (any && m[i] == -INFINITY) l[i] = NAN;
     if (S > 1) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
@@ -1250,7 +1271,7 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
     for (int j = 0; j < 4 * J; ++j) {
       const int d = 4 * kg + 64 * (j / 4) + j % 4;
       const float num = j & 1 ? o[i][j / 2].y : o[i][j / 2].x;
-      if (d < D) out[d * A.os[3]] = m[i] == -INFINITY ? 0.0f : __fdiv_rn(num, l[i]);
+      if (d < D) out[d * A.os[3]] = m[i] == -INFINITY ? l[i] : __fdiv_rn(num, l[i]);
     }
   }
   if (S > 1) {
@@ -1271,14 +1292,18 @@ __global__ void __launch_bounds__(kThreads32, 1) attn_f32_kernel(const __grid_co
       if (r >= rows || d >= D) continue;
       float mx = -INFINITY, num = 0.0f, den = 0.0f;
       for (int k = 0; k < S; ++k) mx = max3(mx, at(k, r, DP), -INFINITY);
-      if (mx != -INFINITY)
-        for (int k = 0; k < S; ++k) {
-          const float pm = at(k, r, DP), f = pm == -INFINITY ? 0.0f : ex2((pm - mx) * cs);
-          num = fmaf(at(k, r, d), f, num);
-          den = fmaf(at(k, r, DP + 1), f, den);
+      for (int k = 0; k < S; ++k) {   // (a part without weights: its sum is 0, or NaN where it had keys)
+        const float pm = at(k, r, DP);
+        if (pm == -INFINITY) {
+          if (mx == -INFINITY) den += at(k, r, DP + 1);
+          continue;
         }
+        const float f = ex2((pm - mx) * cs);
+        num = fmaf(at(k, r, d), f, num);
+        den = fmaf(at(k, r, DP + 1), f, den);
+      }
       ((float*)A.out)[b * A.os[0] + h * A.os[1] + (t0 + r) * A.os[2] + d * A.os[3]] =
-          mx == -INFINITY ? 0.0f : __fdiv_rn(num, den);
+          mx == -INFINITY ? den : __fdiv_rn(num, den);
     }
     __syncwarp();   // no CTA of the cluster leaves while its shared memory is read
     cluster_arrive();

@@ -364,10 +364,12 @@ int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
  * queries' own sequence); query head h reads key head h / (H / Hk), so H is a
  * multiple of Hk.  One dtype for q, k, v and out: float32 or float16; any
  * strides (a permuted [B, T, H, D] projection is read in place; float16 rows
- * off 16-byte boundaries take a slow kernel); D at most 128.  lengths (NULL: Tk): int32 or int64 [B], the keys of each batch entry,
- * clamped to 0..Tk.  key_mask (NULL: none): bool [B, Tk], true where a key
- * takes part.  Keys that do not take part are never looked at, whatever their
- * k and v rows hold; a query row no key takes part in gives zeros.  scale:
+ * off 16-byte boundaries take a slow kernel); D at most 128.  lengths (NULL:
+ * Tk): int32 or int64 [B], the keys of each batch entry, clamped to 0..Tk.
+ * key_mask (NULL: none): bool [B, Tk], true where a key takes part.  Keys that
+ * do not take part are never looked at, whatever their k and v rows hold; a
+ * query row no key takes part in gives zeros, one whose keys all score -inf
+ * NaN (0 / 0), as one with a NaN or +inf score.  scale:
  * positive, at most 2^127 (BT_EINVAL otherwise).  Scores, softmax and sums are
  * float32.
  * replaces: the MatMul, Mul, Add, Softmax, MatMul nodes of an attention block

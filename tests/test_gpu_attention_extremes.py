@@ -98,3 +98,34 @@ def test_large_scores_that_grow_along_the_keys(gpu_runtime, B, H, Hk, Tq, Tk, D,
             q[..., D - 1] = 32.0
             k[..., D - 1] = (step * (torch.arange(Tk, device="cuda") // every)).to(dtype)
             _check(gpu_runtime, q, k, v, f"{sign} {every} {step}")
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,D", FORMS + [(4, 2, 2, Tq, 2500, D) for Tq in (1, 900) for D in (64, 128, 36)])
+def test_scores_of_minus_infinity(gpu_runtime, B, H, Hk, Tq, Tk, D, dtype):
+    """A key that scores -inf has no weight, wherever it lies; where every key
+    that takes part does, the softmax is 0 / 0 and the row NaN; a row no key
+    takes part in stays 0."""
+    rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(Tk + D)
+    q, k, v = (torch.randn(B, h, t, D, generator=g, device="cuda").to(dtype) for h, t in ((H, Tq), (Hk, Tk), (Hk, Tk)))
+    q[..., 0] = 1.0
+    some = torch.rand(B, Tk, generator=g, device="cuda") < 0.5
+    some[:, :Tk // 2] = True     # whole parts of the keys, the first ones too
+    some[:, -1] = False
+    low = k.clone()
+    low[..., 0] = torch.where(some[:, None, :].expand(B, Hk, Tk), float("-inf"), k[..., 0].float()).to(dtype)
+    assert torch.equal(rt.attention(q, low, v), rt.attention(q, k, v, key_mask=~some))
+    assert rt.attention(q, low, v, key_mask=some).isnan().all()
+    n = torch.full((B,), Tk, dtype=torch.int32, device="cuda")
+    n[0], n[1] = Tk // 2, 0
+    o = rt.attention(q, low, v, lengths=n)
+    assert o[0].isnan().all() and (o[1] == 0).all() and torch.isfinite(o[2:]).all()
+    assert (rt.attention(q, low, v, key_mask=torch.zeros_like(some)) == 0).all()
+    # one row of queries
+    row = q.clone()
+    row[0, H - 1, Tq - 1, 0] = float("inf")
+    o = rt.attention(row, torch.cat([-k[..., :1].abs() - 1, k[..., 1:]], -1), v)
+    same = rt.attention(q, torch.cat([-k[..., :1].abs() - 1, k[..., 1:]], -1), v)
+    assert o[0, H - 1, Tq - 1].isnan().all()
+    o[0, H - 1, Tq - 1] = same[0, H - 1, Tq - 1]
+    assert torch.equal(o, same)
