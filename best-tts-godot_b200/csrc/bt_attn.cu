@@ -61,6 +61,15 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// A row's result is a mean of float16 values, so never larger than they are;
+// but rounded weights over an unrounded sum (up to 2^-11 of it) or a long
+// float32 sum may put it past the largest one's rounding range.  Only an
+// infinity among the values is one in the result.
+__device__ __forceinline__ __half half_mean(float y) {
+  const float a = fabsf(y);
+  return __float2half_rn(a > 65504.0f && a < INFINITY ? copysignf(65504.0f, y) : y);
+}
+
 // One warp per query row, any strides: a lane scores one key of 32, then the
 // lanes share the output's dimensions.
 constexpr int kRowWarps = 4;
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
     for (int i = 0; i < kMaxHeadDim / 32; ++i)
       if (lane + 32 * i < A.D) {
         const float y = any ? __fdiv_rn(o[i], l) : 0.0f;
-        if constexpr (sizeof(T) == 2) op[(lane + 32 * i) * A.os[3]] = __float2half_rn(y);
+        if constexpr (sizeof(T) == 2) op[(lane + 32 * i) * A.os[3]] = half_mean(y);
         else op[(lane + 32 * i) * A.os[3]] = y;
       }
   }
@@ -260,6 +269,19 @@ struct Items {
     n_next = it + gridDim.x < A.items ? (int)keys_of(A.a, b2) : 0;
   }
 };
+
+// A warp's rows again, where a result overflowed (see half_mean): into `at`,
+// `step` apart, or, with swizzle >= 0, a staged row whose 16-byte pieces lie
+// at their index xor swizzle.  A call, so that it costs the walk of the items
+// next to nothing (inlined, 64 x 12 heads over 510 keys took 88.0 us against
+// 86.8, and 86.1 without the test for overflows).
+__device__ __noinline__ void store_overflows(uint32_t op, float inv, bool mine, int D, __half* at, int64_t step, int swizzle) {
+#pragma unroll 1
+  for (int i = 0; i < D; ++i) {
+    const float y = tmem_ld1(op + i) * inv;
+    if (mine && fabsf(y) > 65504.0f && fabsf(y) < INFINITY) at[swizzle < 0 ? i * step : i ^ swizzle << 3] = half_mean(y);
+  }
+}
 
 template <int DP>
 __global__ void __launch_bounds__(kAttnThreads, 1)
@@ -459,6 +481,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_wait(pv_done + 2 * tile + ((g - 1) & 1), (g - 1) >> 1 & 1, aborted);
         tc_fence_after();
       }
+      uint32_t over[2] = {};   // NaN once a result is not finite (infinity times 0)
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
         if (32 * i >= a.D) break;
@@ -474,6 +497,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           const __half2 h = none ? __floats2half2_rn(0.0f, 0.0f)
                                         : __floats2half2_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
           y[j] = *reinterpret_cast<const uint32_t*>(&h);
+          asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(over[j & 1]) : "r"(y[j]), "r"(0u));
         }
         if (Sh::kStage && A.wide == 2) {
           // a row of 128 bytes, its 16-byte pieces where the store's swizzle
@@ -502,6 +526,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               if (j < left) out[(int64_t)(32 * i + j) * a.os[3]] = e[j];
           }
         }
+      }
+      if (__any_sync(0xffffffffu, ((over[0] | over[1]) & 0x7fff7fffu) != 0)) {
+        const int row = (warp & 3) * 32 + lane;
+        const bool staged = Sh::kStage && A.wide == 2;
+        store_overflows(op, inv, !none && (staged || t < a.Tq), a.D,
+                        staged ? reinterpret_cast<__half*>(smem + (2 + Sh::kSlots + tile) * Sh::kRows + row * 128) : out,
+                        a.os[3], staged ? row & 7 : -1);
       }
       if (Sh::kStage && A.wide == 2) {
         fence_async_shared();
@@ -744,7 +775,7 @@ __device__ __forceinline__ void few_join(const AttnArgs& A, float* sm, int S, in
       }
     const float y = mx == -INFINITY ? den : num / (den * lift);
     T* out = (T*)A.out + b * A.os[0] + (hk * A.G + gr / A.Tq) * A.os[1] + gr % A.Tq * A.os[2];
-    if constexpr (sizeof(T) == 2) out[d * A.os[3]] = __float2half_rn(y);
+    if constexpr (sizeof(T) == 2) out[d * A.os[3]] = half_mean(y);
     else out[d * A.os[3]] = y;
   }
   if (S > 1) {   // no CTA of the cluster leaves while its shared memory is read

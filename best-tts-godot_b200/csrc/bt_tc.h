@@ -166,6 +166,14 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
       : "r"(addr));
 }
 
+__device__ __forceinline__ float tmem_ld1(uint32_t addr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(r) : "r"(addr));
+  tc_wait_ld();
+  asm volatile("" : "+r"(r)::"memory");
+  return __uint_as_float(r);
+}
+
 // 32 columns of this warp's 32 lanes, written.
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(

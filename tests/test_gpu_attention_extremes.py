@@ -129,3 +129,24 @@ def test_scores_of_minus_infinity(gpu_runtime, B, H, Hk, Tq, Tk, D, dtype):
     assert o[0, H - 1, Tq - 1].isnan().all()
     o[0, H - 1, Tq - 1] = same[0, H - 1, Tq - 1]
     assert torch.equal(o, same)
+
+
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,D", FORMS)
+def test_largest_half_values(gpu_runtime, B, H, Hk, Tq, Tk, D):
+    """A mean of values at the type's largest stays there, also where fifteen
+    weights of sixteen are rounded up by nearly half a step: 2^7 e^-0.6926 =
+    64.035, which float16 holds as 64.0625."""
+    q = torch.zeros(B, H, Tq, D, device="cuda").half()
+    k = torch.zeros(B, Hk, Tk, D, device="cuda").half()
+    q[..., 0], k[..., 0] = 1.0, -1.0
+    k[:, :, ::16, 0] = 0.0
+    v = torch.full_like(k, torch.finfo(F16).max)
+    v[..., 1] *= -1
+    v[..., 2] = 1.0
+    _check(gpu_runtime, q, k, v, "largest values", scale=0.6926)
+    v[:, :, Tk // 2, 3] = float("inf")
+    o = gpu_runtime.attention(q, k, v, scale=0.6926)
+    assert (o[..., 3] == float("inf")).all() and torch.isfinite(o[..., :3]).all()
+    v[:, :, Tk // 2, 3] = float("-inf")
+    o = gpu_runtime.attention(q, k, v, scale=0.6926)
+    assert (o[..., 3] == float("-inf")).all() and torch.isfinite(o[..., :3]).all()
