@@ -296,9 +296,13 @@ class BtRuntime:
 
     def _copy_desc(self, src_desc, src_dt, out):
         """IDENTITY from a source descriptor (any strides, negative ones
-        included) into the tensor view `out`, converting to out's dtype."""
+        included) into the tensor view `out`, converting to out's dtype, on
+        this runtime's device."""
         if out.numel() == 0:
             return out
+        if _get_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self._copy_desc(src_desc, src_dt, out)
         descs = (_lib.BtTensor * 1)(src_desc)
         cdt = self._copy_compute(np.result_type(src_dt, np_dtype(out)))
         attrs = _lib.BtEwAttrs(_lib.NP_TO_BT[np.dtype(cdt)], 0.0)
