@@ -350,7 +350,7 @@ int bt_quantize_rows(const bt_tensor* x, const bt_tensor* q,
  * float16 [..., N].  The sum is an exact int32; it is converted to float32,
  * scaled, biased, and rounded to float16 once where out is float16.  K at
  * most 131071 (beyond it the sum could overflow: BT_ETOOBIG); K = 0 gives
- * the bias, or 0.  The rows of a and w start on 16-byte boundaries, each row
+ * the bias, or 0, whatever the scales.  The rows of a and w start on 16-byte boundaries, each row
  * a place of its own (BT_EUNSUPPORTED otherwise).
  * No counterpart in the reference, whose MatMulInteger nodes have one
  * activation scale for the whole tensor. */
