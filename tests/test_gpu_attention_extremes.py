@@ -150,3 +150,26 @@ def test_largest_half_values(gpu_runtime, B, H, Hk, Tq, Tk, D):
     v[:, :, Tk // 2, 3] = float("-inf")
     o = gpu_runtime.attention(q, k, v, scale=0.6926)
     assert (o[..., 3] == float("-inf")).all() and torch.isfinite(o[..., :3]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("B,H,Hk,Tq,Tk,D", FORMS)
+def test_large_scores_under_masks(gpu_runtime, B, H, Hk, Tq, Tk, D, dtype):
+    """Rows near 2e8 beside rows of small scores, over the keys that take part."""
+    rt, g = gpu_runtime, torch.Generator("cuda").manual_seed(Tq + Tk + D)
+    q, k = _whole(g, 2, (B, H, Tq, D), dtype), _whole(g, 2, (B, Hk, Tk, D), dtype)
+    q[:, ::2] *= 8192
+    q[:, :, ::3] *= 0.125
+    k *= 16
+    v = torch.randn(B, Hk, Tk, D, generator=g, device="cuda").to(dtype)
+    keep = torch.rand(Tk, generator=g, device="cuda") < 0.6
+    keep[:min(Tk // 3, 140)] = False
+    n = Tk - 13
+    live = keep.nonzero()[:, 0]
+    live = live[live < n]
+    want = attention_of_exact_scores(q, k[:, :, live], v[:, :, live])
+    out = torch.ones(Tk, dtype=torch.bool, device="cuda")
+    out[live] = False
+    k, v = (t.masked_fill(out[:, None], float("nan")) for t in (k, v))
+    o = rt.attention(q, k, v, lengths=torch.full((B,), n, dtype=torch.int32, device="cuda"), key_mask=keep.expand(B, Tk))
+    assert_within(o, *want)
