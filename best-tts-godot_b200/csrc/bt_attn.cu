@@ -153,12 +153,13 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // (D = 64) or 1024 (D = 128), and with two warps a scheduler the latencies
 // between them show.  So tile 0 and 1 take turns at the exponentials (each
 // then has the special-function unit to itself while the other waits, reads
-// and compares: 134 -> 120 us at 16 heads of 4096 x 4096 x 64).  There, and at
-// D = 128, 120 and 151 us are 575 and 909 TFLOP/s.  Measured and not taken:
-// blocks of 64 keys with two score buffers a tile (174 us: each block has a
-// fixed part), two threads a row (144 us), scores read twice instead of kept
-// (157 us), the maximum found along with the weights and these redone where it
-// grew (162 us).
+// and compares: 134 -> 120 us at 16 heads of 4096 x 4096 x 64).  Measured
+// beside those 120 us and not taken: blocks of 64 keys with two score buffers a
+// tile (174 us: each block has a fixed part), two threads a row (144 us),
+// scores read twice instead of kept (157 us), the maximum found along with the
+// weights and these redone where it grew (162 us).  There it takes 111 us now,
+// 617 TFLOP/s, and at D = 128 136 us, 1.01 PFLOP/s, at 1965 MHz (149 us after
+// seconds at the power limit, at 1790 MHz).
 //
 // Softmax: with c = scale log2(e) and a reference value m per row,
 // p = 2^(s c - m c + 7).  m is the row's running maximum, but it moves (and O
@@ -168,8 +169,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(AttnArgs A, i
 // weight loses precision only below 2^-21 of the reference.  The exponent is
 // one fma of the score with 7 - m c, whose rounding is an error of up to 2^-14
 // while m c is below 2^11, and grows with it: to a factor past float16's range
-// at 2^24.  A row beyond 2^11 subtracts m from its scores first (a vote a key
-// tile and, in warps with such a row, a pass over the scores).  P is rounded to
+// at 2^24.  A row beyond 2^11 subtracts m from its scores first: a vote a key
+// tile (4096 queries of 16 heads over 16384 keys of 128: 489 -> 496 us), and in
+// warps with such a row a pass over the scores (590 us if every warp made it,
+// as a part of the exponents).  P is rounded to
 // float16 (the tensor cores' operand; relative error 2^-11 a weight, as a
 // float16 result has anyway); the row's sum is of the float32 weights.
 constexpr int kTile = 128;

@@ -63,9 +63,9 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* x
 // the CTA) hold it in registers as V 16-byte vectors each, up to
 // TPR * V * 16 bytes; the at most seven values past the last whole vector
 // are one more value on each of the first lanes.  HBM-bound: 32640 rows of
-// 2048 float32 take 48 us of device time, of float16 30 us (82 us for the
-// float32 rows by the kernel above, which reads them twice and serves longer
-// and unaligned rows).
+// 2048 float32 (334 MB) take 52 us of device time, of float16 (201 MB) 30 us,
+// the rate of a copy (82 us for the float32 rows by the kernel above, which
+// reads them twice and serves longer and unaligned rows).
 template <typename T>
 __device__ __forceinline__ void vec_floats(const uint4 v, float (&f)[16 / sizeof(T)]) {
   if constexpr (sizeof(T) == 2) {
@@ -162,8 +162,13 @@ void quantize_run(const T* x, int64_t ldx, int64_t rows, int64_t K, int8_t* q, i
     return;
   }
   // a warp a row where its registers hold the row and there are rows enough
-  // for eight CTAs on every SM; else a CTA a row (510 rows of 2048 float32:
-  // 4.1 us, by warps 5.1 us; 32640 rows: 48 us by warps)
+  // for eight CTAs on every SM; else a CTA a row (rows of 2048 float32, us of
+  // device time by warps / CTAs: 510 rows 3.2 / 2.8, 2400 rows 6.3 / 7.1, 32640
+  // rows 52 / 77).  Of the kernels whose registers hold the row, the one with the
+  // fewest vectors a thread: 32640 rows of 256 float32 with 2 / 6 vectors 9.2 /
+  // 11.7 us, of 768 with 6 / 8 / 16 17.7 / 18.6 / 28.8, of 1024 with 8 / 16 22.6 /
+  // 30.2; by CTAs 510 rows of 768 with 1 / 4 2.3 / 2.6, 2000 rows of 4096 with
+  // 4 / 8 / 16 7.9 / 8.9 / 14.9.
   const bool warp = row_bytes <= 32 * 16 * 16 && rows > 8 * sms;
   const int tpr = warp ? 32 : 256, per = (int)((row_bytes + tpr * 16 - 1) / (tpr * 16));
   const int64_t want = warp ? (rows + 7) / 8 : rows, cap = (int64_t)sms * 8;
@@ -218,11 +223,14 @@ __global__ void __launch_bounds__(256) matmul_empty_kernel(MmArgs A) {
 // 128-byte-wide blocks of both operands by TMA into a ring of stages (the
 // pair splits the tokens, so each SM loads and reads half of them), warp 1
 // issues the matrix instructions, sixteen further warps scale and store from
-// one of two accumulators while the next tile fills the other.  That pass is
-// bound by its chain of steps, not by the stores: with eight warps the
-// batched projection (32640 x 2048 x 768, float16) took 69 us, and turning
-// the tile round in shared memory for whole-row or TMA stores changed
-// nothing (67-71 us).
+// one of two accumulators while the next tile fills the other.  What bounds a
+// batched projection (32640 x 2048 x 768, us of device time, float16 / float32
+// results): loads and products alone take 36 / 36, with the sums read and
+// scaled but not stored 43 / 43, with the stores (134, 267 MB) 60 / 74: they
+// overlap the rest only in part, and the storing warps wait longest at the
+// release of an accumulator, which comes after its stores.  With eight storing
+// warps instead of sixteen float16 took 69 us; whole-row and TMA stores from
+// shared memory were measured with those eight only (67-71 us).
 //
 // Where a product has fewer tiles than the GPU has SMs, S CTAs form a cluster
 // that splits the summed axis of one tile; each sends its int32 partial sums
@@ -593,10 +601,23 @@ int mm_launch(const MmArgs& A, int S, int sms, const char* what) {
 // The tile and the split with the least estimated time, in SM clocks: a block
 // of 128 along the summed axis takes the longer of its matrix instructions
 // (8192 products a clock) and its loads (64 bytes a clock); a tile adds its
-// stores, a launch its start, a split its exchange.  Device times, us, of M x N
-// x K (graphs of 20 launches):
-//   split / not:   64 x 4096 x 4096   11.0 / 12.5;   1 x 8192 x 8192  14.8 / 21.0
-//   pair / single: 4096 x 4096 x 4096 49.9 / 51.6;   32640 x 2048 x 768 59.7 / 58.8
+// stores, a launch its start, a split its exchange.  The estimates are there to
+// be compared: they leave out most of what loads from cold and stores take, and
+// come to half the time that is measured.  Their choice against every other
+// tile and split, us of device time, as tokens of a tile / split (p: a pair):
+//   M x N x K              chosen           the others' best
+//   1 x 2048 x 768         16/1     5.3     16/6    6.4
+//   1 x 8192 x 8192        16/2    18.1     16/1   22.3
+//   16 x 768 x 768         16/1     5.3     16/6    7.5
+//   64 x 4096 x 4096       64/4    11.1     64/3   12.1    (without a split 12.7)
+//   77 x 5001 x 1000       32/1     6.3     64/1    7.0    (with a split 12.3)
+//   300 x 3001 x 5120      64/1    16.0     128/1  16.9    (with a split 20.8)
+//   510 x 768 x 2048       32/1     8.1     64/1    8.9    (with a split 12.4)
+//   510 x 2048 x 768       64/1     6.1     128/1   6.9
+//   2048 x 2048 x 512      256p     8.7     256/1   8.0
+//   4096 x 4096 x 4096     256p    55       256/1  60
+//   8160 x 768 x 2048      256p    19.8     256/1  20.3
+//   32640 x 2048 x 768     256p    60       256/1  59      (float32 results: 75, 72)
 struct MmChoice {
   int64_t M, N, K;
   int sms, nt, cg, split;
