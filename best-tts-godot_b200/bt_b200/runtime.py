@@ -945,7 +945,7 @@ class BtRuntime:
         entry (default: all); key_mask: bool [B, Tk], true where a key takes
         part; keys that do not are never looked at, and a row without any
         gives zeros (one whose keys all score -inf NaN).  scale, above 0 and up
-        to 2^127, defaults to 1 / sqrt(D).  Views of any strides
+        to 2.35e38, defaults to 1 / sqrt(D).  Views of any strides
         are read in place (a [B, T, H, D] projection permuted to
         [B, H, T, D]), except that long float16 ones whose rows do not start
         on 16-byte boundaries are copied to such rows first."""

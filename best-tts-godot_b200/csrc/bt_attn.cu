@@ -1496,8 +1496,8 @@ extern "C" int bt_attention(const bt_tensor* q, const bt_tensor* k, const bt_ten
   if (Hk < 1 ? A.H != 0 : A.H % Hk != 0)
     return set_error(BT_ESHAPE, "%s: %lld query heads cannot share %lld key heads", what, (long long)A.H, (long long)Hk);
   if (D < 1 || D > kMaxHeadDim) return set_error(BT_ETOOBIG, "%s: dim %lld outside 1..%d", what, (long long)D, kMaxHeadDim);
-  if (!(scale > 0.0f) || scale > 0x1p127f)   // (scale log2(e) is finite)
-    return set_error(BT_EINVAL, "%s: scale must be positive and at most 2^127", what);
+  if (!(scale > 0.0f) || isinf(scale * 1.4426950408889634f))   // (the kernels' scale log2(e))
+    return set_error(BT_EINVAL, "%s: scale must be positive and scale log2(e) finite", what);
   if (A.Tk > INT32_MAX / 2 || A.Tq > INT32_MAX / 2) return set_error(BT_ETOOBIG, "%s: more than 2^30 positions", what);
   if (lengths) {
     if ((rc = check_tensor(lengths, "lengths", false))) return rc;

@@ -369,10 +369,10 @@ int bt_matmul_int8(const bt_tensor* a, const bt_tensor* a_scale,
  * key_mask (NULL: none): bool [B, Tk], true where a key takes part.  Keys that
  * do not take part are never looked at, whatever their k and v rows hold; a
  * query row no key takes part in gives zeros, one whose keys all score -inf
- * NaN (0 / 0), as one with a NaN or +inf score.  scale:
- * positive, at most 2^127 (BT_EINVAL otherwise).  Scores, softmax and sums are
- * float32 (a float32 row's sum of |v| over its keys has to stay in range);
- * float16 inputs round each weight to float16.
+ * NaN (0 / 0), as one with a NaN or +inf score.  scale: positive, and scale
+ * log2(e) finite, which it is up to 2.35e38 (BT_EINVAL otherwise).  Scores,
+ * softmax and sums are float32 (a float32 row's sum of |v| over its keys has to
+ * stay in range); float16 inputs round each weight to float16.
  * replaces: the MatMul, Mul, Add, Softmax, MatMul nodes of an attention block
  *           (ref_runtime.py:446-451, :269-273 + :599-600 for Mul, Add and
  *           Softmax), one dispatch each in the reference. */
